@@ -45,6 +45,7 @@ import threading
 import torch
 
 DTYPES = {torch.float32: 0, torch.bfloat16: 1}
+FP8 = torch.float8_e4m3fn  # the 8-bit cache's codes
 HEAD_DIMS = (32, 64, 128)
 _DIR = os.path.dirname(os.path.abspath(__file__))
 LIBRARY = "libcpu_attention_hip.so"
@@ -96,8 +97,35 @@ class FlashArgs(ctypes.Structure):
     ]
 
 
+class FlashWindowArgs(ctypes.Structure):
+    """``ca_flash_window_args`` (include/cpu_attention_hip.h)."""
+    _fields_ = [("flash", FlashArgs), ("left", ctypes.c_int64), ("right", ctypes.c_int64),
+                ("sinks", ctypes.c_int64)]
+
+
+class DecodeWindowArgs(ctypes.Structure):
+    """``ca_decode_window_args`` (include/cpu_attention_hip.h)."""
+    _fields_ = [("decode", DecodeArgs), ("k_scale", ctypes.c_void_p), ("v_scale", ctypes.c_void_p),
+                ("left", ctypes.c_int64), ("sinks", ctypes.c_int64)]
+
+
+class StoreFp8Args(ctypes.Structure):
+    """``ca_store_fp8_args`` (include/cpu_attention_hip.h)."""
+    _fields_ = [("store", StoreArgs), ("k_scale", ctypes.c_void_p), ("v_scale", ctypes.c_void_p),
+                ("workspace", ctypes.c_void_p), ("workspace_bytes", ctypes.c_int64)]
+
+
+class CopyBlocksArgs(ctypes.Structure):
+    """``ca_copy_blocks_args`` (include/cpu_attention_hip.h)."""
+    _fields_ = [("arrays", ctypes.POINTER(ctypes.c_void_p)), ("num_arrays", ctypes.c_int64),
+                ("block_bytes", ctypes.c_int64), ("mapping", ctypes.c_void_p),
+                ("num_pairs", ctypes.c_int64), ("num_blocks", ctypes.c_int64)]
+
+
 EXPORTS = ("ca_store", "ca_decode", "ca_decode_noalloc", "ca_decode_workspace_bytes", "ca_flash",
-           "ca_flash_workspace_bytes", "ca_abi_version", "ca_version", "ca_status_string")
+           "ca_flash_workspace_bytes", "ca_flash_window", "ca_flash_window_workspace_bytes",
+           "ca_decode_window", "ca_decode_window_workspace_bytes", "ca_store_fp8",
+           "ca_store_fp8_workspace_bytes", "ca_copy_blocks", "ca_abi_version", "ca_version", "ca_status_string")
 
 _HOST_CHECKS = [os.environ.get("CPU_ATTENTION_HOST_CHECKS", "1") != "0"]
 
@@ -137,6 +165,16 @@ def load_library(path=None):
     lib.ca_flash.restype = ctypes.c_int
     lib.ca_flash_workspace_bytes.argtypes = [i64, i64, i64, i64, i64, i32]
     lib.ca_flash_workspace_bytes.restype = i64
+    for entry, args in (("ca_flash_window", FlashWindowArgs), ("ca_decode_window", DecodeWindowArgs),
+                        ("ca_store_fp8", StoreFp8Args), ("ca_copy_blocks", CopyBlocksArgs)):
+        getattr(lib, entry).argtypes = [ctypes.POINTER(args), vp]
+        getattr(lib, entry).restype = ctypes.c_int
+    lib.ca_flash_window_workspace_bytes.argtypes = [i64, i64, i64, i64, i64, i32, i32, i64, i64, i64]
+    lib.ca_flash_window_workspace_bytes.restype = i64
+    lib.ca_decode_window_workspace_bytes.argtypes = [i64] * 7
+    lib.ca_decode_window_workspace_bytes.restype = i64
+    lib.ca_store_fp8_workspace_bytes.argtypes = [i64] * 3
+    lib.ca_store_fp8_workspace_bytes.restype = i64
     lib.ca_abi_version.argtypes = []
     lib.ca_abi_version.restype = ctypes.c_int
     lib.ca_version.argtypes = []
@@ -448,18 +486,187 @@ class Module:
         return out
 
 
+    # -- window and sinks, the 8-bit cache, copies of pages ---------------------
+    def _scales_ok(self, k_scale, v_scale, k_cache):
+        """An 8-bit cache's scales: fp32 ``[blocks, heads]``, contiguous, two tensors."""
+        for t in (k_scale, v_scale):
+            if not _plain(t) or t.dim() != 2 or t.dtype != torch.float32 or tuple(t.shape) != tuple(k_cache.shape[:2]) \
+                    or not t.is_contiguous() or not _on_gpu(k_cache.device, t):
+                return False
+        return k_scale.numel() == 0 or k_scale.data_ptr() != v_scale.data_ptr()
+
+    def _scratch(self, nbytes, device):
+        return torch.empty(nbytes, dtype=torch.uint8, device=device) if nbytes > 0 else None
+
+    def flash_window(self, rt, q, k, v, scale, causal, left, right, sinks):
+        """flash_attn_window_func over q/k/v as ``flash`` takes them. Returns the
+        output, or None."""
+        if not (_plain(q) and _plain(k) and _plain(v)):
+            return None
+        qsh, ksh = q.shape, k.shape
+        if len(qsh) != 4 or len(ksh) != 4 or v.shape != ksh:
+            return None
+        b, sq, heads, hd = qsh
+        sk, dt = ksh[1], q.dtype
+        if dt not in DTYPES or hd not in HEAD_DIMS or sq < 1 or sk < 1:
+            return None
+        if ksh[0] != b or ksh[2] != heads or ksh[3] != hd or k.dtype != dt or v.dtype != dt:
+            return None
+        if q.stride(3) != 1 or k.stride(3) != 1 or v.stride(3) != 1 or not (causal is True or causal is False):
+            return None
+        dev = q.device
+        if not q.is_cuda or not _on_gpu(dev, k, v):
+            return None
+        with torch.cuda.device(dev):
+            ws = self._scratch(self.lib.ca_flash_window_workspace_bytes(
+                b, sq, sk, heads, hd, DTYPES[dt], 1 if causal else 0, left, right, sinks), dev)
+            out = torch.empty(qsh, dtype=dt, device=dev)
+            args = FlashWindowArgs(
+                FlashArgs(q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(), b, sq, sk, heads, hd,
+                          _strides3(q.stride(), qsh), _strides3(k.stride(), ksh), _strides3(v.stride(), ksh),
+                          float(hd) ** -0.5 if scale is None else float(scale), 1 if causal else 0, DTYPES[dt], 0,
+                          ws.data_ptr() if ws is not None else None, ws.numel() if ws is not None else 0),
+                left, right, sinks)
+            rc = self.lib.ca_flash_window(ctypes.byref(args), _stream(dev))
+        if rc == CA_DECLINED:
+            return None
+        if rc != CA_OK:
+            self._raise(rc, "flash_window")
+        return out
+
+    def decode_window(self, rt, q, k_cache, v_cache, k_scale, v_scale, k, v, lens, page_table, scale, left, sinks, n):
+        """Paged decode of q ``[seqs, (1,) heads, dim]`` with a window and sinks, over
+        the cache of q's type (scales None) or the 8-bit one; with k/v, ``n`` new
+        tokens per sequence (rows ``[seqs * n, heads, dim]``, or q's shape for n = 1)
+        are appended at ``lens`` first. Returns the output, or None."""
+        if not (_plain(q) and _plain(page_table)) or n < 1 or q.dim() not in (3, 4) \
+                or (q.dim() == 4 and q.shape[1] != 1):
+            return None
+        b, heads, hd = q.shape[0], q.shape[-2], q.shape[-1]
+        dt = q.dtype
+        if dt not in DTYPES or hd not in HEAD_DIMS or not _rows_ok(q, hd):
+            return None
+        fp8 = k_scale is not None
+        if not _caches_ok(k_cache, v_cache, FP8 if fp8 else dt, heads, hd):
+            return None
+        if page_table.dim() != 2 or page_table.dtype != torch.int32 or page_table.shape[0] != b \
+                or not page_table.is_contiguous() or not _int_vector(lens, torch.int32, b):
+            return None
+        dev = q.device
+        if not q.is_cuda or not _on_gpu(dev, k_cache, v_cache):
+            return None
+        if not self._scales_ok(k_scale, v_scale, k_cache) if fp8 else v_scale is not None:
+            return None
+        store = k is not None
+        if store:
+            if not (_plain(k) and _plain(v)) or tuple(k.shape) != (tuple(q.shape) if n == 1 else (b * n, heads, hd)) \
+                    or v.shape != k.shape or v.stride() != k.stride() or k.dtype != dt or v.dtype != dt \
+                    or not _rows_ok(k, hd) or not _on_gpu(dev, k, v):
+                return None
+        elif v is not None:
+            return None
+        page, width = k_cache.shape[2], page_table.shape[1]
+        if _HOST_CHECKS[0] and b and int(lens.max()) + (n if store else 0) > width * page:
+            return None
+        with torch.cuda.device(dev):
+            lens, page_table = _index_on(lens, dev), _index_on(page_table, dev)
+            out = torch.empty(q.shape, dtype=dt, device=dev)
+            ws = self._scratch(self.lib.ca_decode_window_workspace_bytes(b, heads, hd, page, width, left, sinks), dev)
+            args = DecodeWindowArgs(
+                DecodeArgs(q.data_ptr(), _stride(q, 0), k_cache.data_ptr(), v_cache.data_ptr(),
+                           k.data_ptr() if store else None, v.data_ptr() if store else None,
+                           _stride(k, 0) if store else 0, None, lens.data_ptr(), page_table.data_ptr(), width,
+                           out.data_ptr(), b, heads, hd, page, k_cache.shape[0],
+                           float(hd) ** -0.5 if scale is None else float(scale), DTYPES[dt],
+                           ws.data_ptr() if ws is not None else None, ws.numel() if ws is not None else 0,
+                           n if store else 0),
+                k_scale.data_ptr() if fp8 else None, v_scale.data_ptr() if fp8 else None, left, sinks)
+            rc = self.lib.ca_decode_window(ctypes.byref(args), _stream(dev))
+        if rc == CA_DECLINED:
+            return None
+        if rc != CA_OK:
+            self._raise(rc, "decode_window")
+        return out
+
+    def store_fp8(self, rt, key, value, k_cache, v_cache, k_scale, v_scale, slots):
+        """``reshape_and_cache_fp8``. True, or None."""
+        if not (_plain(key) and _plain(value)) or key.dim() != 3 or value.dim() != 3:
+            return None
+        n, heads, hd = key.shape
+        if key.dtype not in DTYPES or hd not in HEAD_DIMS or value.dtype != key.dtype or not _rows_ok(key, hd) \
+                or value.shape != key.shape or value.stride() != key.stride():
+            return None
+        if not _caches_ok(k_cache, v_cache, FP8, heads, hd) or not _int_vector(slots, torch.int64, n):
+            return None
+        dev = k_cache.device
+        if not k_cache.is_cuda or not _on_gpu(dev, v_cache, key, value) \
+                or not self._scales_ok(k_scale, v_scale, k_cache) \
+                or (k_cache.numel() and k_cache.data_ptr() == v_cache.data_ptr()):
+            return None
+        page, nblocks = k_cache.shape[2], k_cache.shape[0]
+        if _HOST_CHECKS[0] and n and int(slots.max()) >= nblocks * page:
+            return None
+        if n == 0 or nblocks == 0:
+            return True
+        with torch.cuda.device(dev):
+            slots = _index_on(slots, dev)
+            ws = self._scratch(self.lib.ca_store_fp8_workspace_bytes(n, nblocks, page), dev)
+            args = StoreFp8Args(
+                StoreArgs(key.data_ptr(), value.data_ptr(), _stride(key, 0), k_cache.data_ptr(), v_cache.data_ptr(),
+                          slots.data_ptr(), n, heads, hd, page, nblocks, DTYPES[key.dtype], 0),
+                k_scale.data_ptr(), v_scale.data_ptr(), ws.data_ptr() if ws is not None else None,
+                ws.numel() if ws is not None else 0)
+            rc = self.lib.ca_store_fp8(ctypes.byref(args), _stream(dev))
+        if rc == CA_DECLINED:
+            return None
+        if rc != CA_OK:
+            self._raise(rc, "store_fp8")
+        return True
+
+    def copy_blocks(self, rt, arrays, mapping):
+        """Pages ``mapping[i][0]`` -> ``mapping[i][1]`` (int64 ``[pairs, 2]``) within each
+        tensor of the list ``arrays`` (contiguous, the same shape and type, pages
+        along dim 0). True, or None."""
+        if not isinstance(arrays, list) or not _plain(mapping) or mapping.dim() != 2 or mapping.shape[1] != 2 \
+                or mapping.dtype != torch.int64 or not mapping.is_contiguous():
+            return None
+        if not arrays:
+            return True
+        first = arrays[0]
+        for t in arrays:
+            if not _plain(t) or t.dim() < 1 or not t.is_contiguous() or t.shape != first.shape \
+                    or t.dtype != first.dtype or not t.is_cuda or t.device != first.device:
+                return None
+        if mapping.shape[0] == 0 or first.numel() == 0:
+            return True
+        dev = first.device
+        with torch.cuda.device(dev):
+            mapping = _index_on(mapping, dev)
+            ptrs = (ctypes.c_void_p * len(arrays))(*[t.data_ptr() for t in arrays])
+            args = CopyBlocksArgs(ptrs, len(arrays), first.numel() * first.element_size() // first.shape[0],
+                                  mapping.data_ptr(), mapping.shape[0], first.shape[0])
+            rc = self.lib.ca_copy_blocks(ctypes.byref(args), _stream(dev))
+        if rc == CA_DECLINED:
+            return None
+        if rc != CA_OK:
+            self._raise(rc, "copy_blocks")
+        return True
+
+
 def _stream_of_index(index):
     return torch.cuda.current_stream(index).cuda_stream
 
 
 class NativeModule(Module):
-    """``Module`` with decode/store/flash's argument handling in the native
+    """``Module`` with the entries' argument handling in the native
     extension ``_binding`` (csrc/ca_binding.cpp): the same rules in the same
     order, the same results.  The entries are the extension's functions
     themselves, so a call runs no Python code of this package."""
 
     ENTRIES = ("ca_decode", "ca_store", "ca_flash", "ca_decode_workspace_bytes",
-               "ca_flash_workspace_bytes", "ca_status_string")
+               "ca_flash_workspace_bytes", "ca_status_string", "ca_flash_window",
+               "ca_flash_window_workspace_bytes", "ca_decode_window", "ca_decode_window_workspace_bytes",
+               "ca_store_fp8", "ca_store_fp8_workspace_bytes", "ca_copy_blocks")
 
     def __init__(self, lib, binding):
         super().__init__(lib)
@@ -469,6 +676,10 @@ class NativeModule(Module):
         self.decode = binding.decode
         self.store = binding.store
         self.flash = binding.flash
+        self.flash_window = binding.flash_window
+        self.decode_window = binding.decode_window
+        self.store_fp8 = binding.store_fp8
+        self.copy_blocks = binding.copy_blocks
 
     def _decode(self, q, k_cache, v_cache, k, v, slots, lens, page_table, scale, dst, n):
         return self.binding.decode(None, q, k_cache, v_cache, k, v, slots, lens, page_table, scale, dst, n)

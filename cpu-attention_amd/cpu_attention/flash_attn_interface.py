@@ -7,7 +7,9 @@
 """The flash-attn entry points, computed on an MI355X.
 
 ``flash_attn_func`` (dense prefill) and ``flash_attn_with_kvcache`` (paged decode)
-take flash-attn's arguments.  An option this build does not implement is refused
+take flash-attn's arguments; ``flash_attn_window_func`` and
+``flash_attn_window_with_kvcache`` add a sliding window and sinks, and
+``flash_attn_with_kvcache_fp8`` an 8-bit cache.  An option this build does not implement is refused
 with ``NotImplementedError`` rather than ignored.  The fast path hands the
 tensors straight to the kernel module, which checks them itself and returns
 ``None`` for anything its kernels cannot read; only then does this module
@@ -21,15 +23,20 @@ torch's current stream; and an integer ``cache_seqlens`` or the positions of a
 multi-token append are made on the GPU.
 """
 
+import math
+import operator
+
 import torch
 
 from . import _kernel as K
-from .cache import reshape_and_cache
+from .cache import SCALES as _SCALES
+from .cache import check_fp8_cache, reshape_and_cache
 
 _MHA_ONLY = "cpu_attention supports MHA only (nheads == nheads_k); GQA/MQA are not supported yet"
 _DEVICE = "cpu_attention: the MI355X build takes tensors on one ROCm GPU"
 _REFUSED = ("cpu_attention: qv, rotary, cache_leftpad, varlen, descale, sliding "
             "windows, softcap, attention_chunk, alibi and return_softmax_lse are not supported")
+_NEW_TOKENS = "cpu_attention: k/v must both be [batch, seqlen_new, nheads, headdim]"
 _ENTRIES = []  # [runtime handle, module decode, module flash] once the library is loaded
 
 
@@ -296,6 +303,201 @@ def _check_flash(q, k, v):
             x = x.contiguous()
         readable.append(_in_place_or_copy(x, [x.stride(i) if x.shape[i] > 1 else 0 for i in range(3)]))
     return readable
+
+
+def _window_options(window_size, sink_tokens, softmax_scale):
+    """The window's (left, right) and the sinks as whole numbers, checked."""
+    try:
+        left, right = (operator.index(x) for x in window_size)
+        sinks = operator.index(sink_tokens)
+    except (TypeError, ValueError):
+        raise ValueError("cpu_attention: window_size must be two ints and sink_tokens an int") from None
+    if left < -1 or right < -1 or sinks < 0 or max(left, right, sinks) >= 1 << 62:
+        raise ValueError("cpu_attention: window_size must be -1 (no limit) or more on each side, "
+                         "sink_tokens 0 or more")
+    if softmax_scale is not None and not 0.0 < float(softmax_scale) < math.inf:
+        raise ValueError("cpu_attention: softmax_scale must be positive and finite")
+    return left, right, sinks
+
+
+def flash_attn_window_func(q, k, v, window_size=(-1, -1), sink_tokens=0, softmax_scale=None, causal=False):
+    """``flash_attn_func`` with a sliding window and attention sinks, forward only.
+
+    Query ``i`` stands at position ``p = i + seqlen_k - seqlen_q`` (bottom-right
+    aligned) and sees the keys ``p - left .. p + right`` of ``window_size = (left,
+    right)`` and, of the first ``sink_tokens`` keys, those up to ``p + right``.  -1
+    leaves a side open; ``causal`` sets ``right`` to 0.  A query that sees no key gets
+    zeros.  Values of keys that a query does not see never reach it, infinities and NaNs
+    included -- unless the window leaves nothing out of the causal or the full call,
+    which then is ``flash_attn_func``'s.  Shapes, types, strides and errors are
+    ``flash_attn_func``'s; ``softmax_scale`` must be positive and finite.
+    """
+    left, right, sinks = _window_options(window_size, sink_tokens, softmax_scale)
+    flash, rt = K.module().flash_window, K.runtime()
+    out = flash(rt, q, k, v, softmax_scale, causal, left, right, sinks)
+    if out is None:
+        q, k, v = _check_flash(q, k, v)
+        out = flash(rt, q, k, v, softmax_scale, bool(causal), left, right, sinks)
+        if out is None:  # strides past the kernels' 32-bit tile offsets
+            q, k, v = (x.clone(memory_format=torch.contiguous_format) for x in (q, k, v))
+            out = flash(rt, q, k, v, softmax_scale, bool(causal), left, right, sinks)
+        if out is None:
+            raise RuntimeError("cpu_attention: the kernel declined arguments that passed validation")
+    return out
+
+
+def flash_attn_window_with_kvcache(
+    q,
+    k_cache,
+    v_cache,
+    k=None,
+    v=None,
+    cache_seqlens=None,
+    page_table=None,
+    window_size=(-1, -1),
+    sink_tokens=0,
+    softmax_scale=None,
+    cache_batch_idx=None,
+    block_table=None,
+):
+    """``flash_attn_with_kvcache`` with a sliding window and attention sinks.
+
+    The query is the newest of its sequence's ``len`` tokens (the appended ones
+    counted) and sees the keys ``len - 1 - left .. len - 1`` of ``window_size = (left,
+    right)`` (-1: all of them; ``right`` has no effect) and the first ``sink_tokens``
+    keys.  Only those are read: pages that hold none of them need not hold anything,
+    and their page-table entries are not read.  Everything else is
+    ``flash_attn_with_kvcache``'s; ``softmax_scale`` must be positive and finite.
+    """
+    return _decode_window(q, k_cache, v_cache, None, None, k, v, cache_seqlens, page_table, window_size, sink_tokens,
+                          softmax_scale, cache_batch_idx, block_table)
+
+
+def flash_attn_with_kvcache_fp8(
+    q,
+    k_cache,
+    v_cache,
+    k_scale,
+    v_scale,
+    k=None,
+    v=None,
+    cache_seqlens=None,
+    page_table=None,
+    window_size=(-1, -1),
+    sink_tokens=0,
+    softmax_scale=None,
+    cache_batch_idx=None,
+    block_table=None,
+):
+    """``flash_attn_window_with_kvcache`` over an 8-bit cache.
+
+    The caches are ``torch.float8_e4m3fn`` ``[num_blocks, nheads, page_block_size,
+    headdim]`` in this library's layout (K as 32-bit words of 4 neighbouring dims,
+    transposed inside a page), written only by ``reshape_and_cache_fp8`` or by
+    ``k``/``v`` here; ``k_scale`` and ``v_scale`` are fp32 ``[num_blocks, nheads]``, one
+    power of two for each page and head: a code stands for code * scale.  ``q``,
+    ``k``, ``v`` and the output are bf16 or fp32.
+
+    ``k``/``v`` of ``n`` new tokens per sequence are appended as
+    ``reshape_and_cache_fp8`` stores them: the page's scale grows with them and what
+    the page holds is rescaled, so no two sequences of a call may share a page that
+    they append to.
+    """
+    if k_scale is None or v_scale is None:
+        raise ValueError(_SCALES)
+    return _decode_window(q, k_cache, v_cache, k_scale, v_scale, k, v, cache_seqlens, page_table, window_size, sink_tokens,
+                          softmax_scale, cache_batch_idx, block_table)
+
+
+def _decode_window(q, k_cache, v_cache, k_scale, v_scale, k, v, lens, page_table, window_size, sink_tokens, scale,
+                   batch_idx, block_table):
+    """The decode over either cache (scales None: q's type)."""
+    left, _, sinks = _window_options(window_size, sink_tokens, scale)
+    if block_table is not None:
+        if page_table is not None:
+            raise ValueError("cpu_attention: pass `page_table` or `block_table`, not both")
+        page_table = block_table
+    if page_table is None:
+        raise ValueError("cpu_attention: pass `page_table`")
+    if batch_idx is not None:
+        page_table = page_table.index_select(0, batch_idx.to(page_table.device).long())
+    if not isinstance(lens, torch.Tensor):
+        if lens is None:
+            raise ValueError("cpu_attention: `cache_seqlens` is required")
+        where = q.device if isinstance(q, torch.Tensor) else "cpu"
+        lens = torch.full((q.shape[0],), lens, dtype=torch.int32, device=where)
+    n = 1
+    if isinstance(k, torch.Tensor) and isinstance(v, torch.Tensor) and k.dim() == 4 and k.shape[1] != 1:
+        n = k.shape[1]
+        if v.shape != k.shape:
+            raise ValueError(_NEW_TOKENS)
+        if n == 0:  # nothing to append
+            k, v, n = None, None, 1
+        else:  # rows of [seqs * n, heads, dim]
+            k, v = k.reshape(-1, *k.shape[2:]), v.reshape(-1, *v.shape[2:])
+    decode, rt = K.module().decode_window, K.runtime()
+    out = decode(rt, q, k_cache, v_cache, k_scale, v_scale, k, v, lens, page_table, scale, left, sinks, n)
+    if out is None:
+        q, k_cache, v_cache, k_scale, v_scale, k, v, page_table, lens = _check_window_kvcache(
+            q, k_cache, v_cache, k_scale, v_scale, k, v, n, page_table, lens)
+        out = decode(rt, q, k_cache, v_cache, k_scale, v_scale, k, v, lens, page_table, scale, left, sinks, n)
+        if out is None:
+            raise RuntimeError("cpu_attention: the kernel declined arguments that passed validation")
+    return out
+
+
+def _check_window_kvcache(q, k_cache, v_cache, k_scale, v_scale, k, v, n, page_table, lens):
+    """Called once the kernel module declined a decode: ``_check_kvcache``'s rules in its
+    order, with the 8-bit cache's where scales are given.  ``k``/``v``: q's shape for
+    ``n`` = 1, else rows ``[seqs * n, heads, dim]``."""
+    q, k_cache, v_cache, k_scale, v_scale, k, v, page_table, lens = map(
+        _as_plain, (q, k_cache, v_cache, k_scale, v_scale, k, v, page_table, lens))
+    fp8 = k_scale is not None
+    if q.dim() != 4:
+        raise ValueError("cpu_attention: q must be [batch, 1, nheads, headdim]")
+    if q.shape[1] != 1:
+        raise NotImplementedError("cpu_attention decodes one query token per sequence")
+    batch, _, heads, hd = q.shape
+    if k_cache.dim() != 4 or v_cache.shape != k_cache.shape:
+        raise ValueError("cpu_attention: k_cache/v_cache must be "
+                         "[num_blocks, nheads, page_block_size, headdim] and match")
+    if k_cache.shape[3] != hd or k_cache.shape[1] == 0 or heads % k_cache.shape[1]:
+        raise ValueError("cpu_attention: q and the caches disagree on heads or head_dim")
+    if k_cache.shape[1] != heads:
+        raise NotImplementedError(_MHA_ONLY)
+    if not (k_cache.is_contiguous() and v_cache.is_contiguous()):
+        raise ValueError("cpu_attention: the paged caches must be contiguous")
+    if fp8:
+        check_fp8_cache(k_cache, v_cache, k_scale, v_scale)
+        if q.dtype not in K.DTYPES:
+            raise ValueError("cpu_attention: q must be fp32 or bf16")
+    elif q.dtype not in K.DTYPES or k_cache.dtype != q.dtype or v_cache.dtype != q.dtype:
+        raise ValueError("cpu_attention: q and the caches must share a dtype (fp32 or bf16)")
+    if hd not in K.HEAD_DIMS or k_cache.shape[2] == 0 or k_cache.shape[2] % 16:
+        raise ValueError(f"cpu_attention: head_dim must be 32/64/128 (got {hd}) and the "
+                         f"page a multiple of 16 (got {k_cache.shape[2]})")
+    if page_table.dtype != torch.int32 or page_table.dim() != 2 or page_table.shape[0] != batch:
+        raise ValueError("cpu_attention: page_table must be int32 [batch, max_blocks]")
+    if lens.dtype != torch.int32 or lens.shape != (batch,):
+        raise ValueError("cpu_attention: cache_seqlens must be an int or an int32 [batch] tensor")
+    rows = (batch, 1, heads, hd) if n == 1 else (batch * n, heads, hd)
+    if (k is None) != (v is None) or k is not None and (
+            k.shape != rows or v.shape != rows or k.dtype != q.dtype or v.dtype != q.dtype):
+        raise ValueError(_NEW_TOKENS)
+    if batch and int(lens.max()) + (n if k is not None else 0) > page_table.shape[1] * k_cache.shape[2]:
+        raise ValueError("cpu_attention: cache_seqlens exceed the page table's capacity")
+    dev = q.device
+    on_dev = [x for x in (k_cache, v_cache, k_scale, v_scale, k, v) if x is not None]
+    if not q.is_cuda or any(x.device != dev for x in on_dev):
+        raise ValueError(_DEVICE)
+    if not (K.aligned(k_cache) and K.aligned(v_cache)):
+        raise ValueError("cpu_attention: the paged caches must start 16-byte aligned")
+    if k is not None:
+        # k and v must share one layout with packed heads and 16-byte alignment
+        if not (_heads_contiguous(k) is k and v.stride() == k.stride() and K.aligned(v)):
+            k, v = (x.clone(memory_format=torch.contiguous_format) for x in (k, v))
+    return (_heads_contiguous(q), k_cache, v_cache, k_scale, v_scale, k, v, page_table.contiguous(),
+            lens.contiguous())
 
 
 def flash_attn_varlen_func(q, k, v, cu_seqlens_q, cu_seqlens_k, max_seqlen_q,

@@ -292,3 +292,264 @@ extern "C" int ca_flash(const ca_flash_args* a, void* stream) {
   flash_rows_workspace(p, a->workspace, a->workspace_bytes, (int)a->head_dim, a->dtype == CA_BF16);
   return flash_launch(p, (int)a->head_dim, a->dtype == CA_BF16, static_cast<hipStream_t>(stream));
 }
+
+// ---------------------------------------------------------------------------
+// Window and sinks, the 8-bit cache, copies of pages
+// ---------------------------------------------------------------------------
+static bool scale_ok(float scale) { return scale > 0.f && scale < INFINITY; }
+
+// The window in the kernels' terms: no side left open (open: 2^30), and `plain` when it
+// leaves nothing out of the causal (or of the full) call.
+struct WindowSides {
+  int64_t left, right, sinks;
+  bool plain, causal;
+};
+static WindowSides window_sides(int64_t seq_q, int64_t seq_k, bool causal, int64_t left, int64_t right, int64_t sinks) {
+  constexpr int64_t kOpen = 1 << 30;
+  WindowSides w;
+  // The last row stands at seq_k - 1 and sees key 0 with left >= seq_k - 1; the first
+  // at seq_k - seq_q and sees the last key with right >= seq_q - 1.
+  if (causal) right = 0;
+  w.left = left < 0 || left >= seq_k - 1 ? kOpen : left;
+  w.right = right < 0 || right >= seq_q - 1 ? kOpen : right;
+  w.sinks = sinks < 0 ? 0 : (sinks < seq_k ? sinks : seq_k);
+  w.causal = w.right != kOpen;
+  w.plain = w.left == kOpen && (w.right == kOpen || w.right == 0);
+  return w;
+}
+
+static WindowParams window_params(const FlashParams& f, const WindowSides& w) {
+  WindowParams p{};
+  static_cast<FlashParams&>(p) = f;
+  p.left = (int32_t)w.left;
+  p.right = (int32_t)w.right;
+  p.sinks = (int32_t)w.sinks;
+  return p;
+}
+
+extern "C" int64_t ca_flash_window_workspace_bytes(int64_t batch, int64_t seq_q, int64_t seq_k, int64_t num_heads,
+                                                   int64_t head_dim, int32_t dtype, int32_t causal, int64_t left,
+                                                   int64_t right, int64_t sinks) {
+  if (!dtype_ok(dtype) || !head_dim_ok(head_dim) || batch < 1 || num_heads < 1 || seq_q < 1 || seq_k < 1) return 0;
+  if (seq_q >= (1 << 30) || seq_k >= (1 << 30)) return 0;  // declined
+  const WindowSides w = window_sides(seq_q, seq_k, causal != 0, left, right, sinks);
+  if (w.plain) return ca_flash_workspace_bytes(batch, seq_q, seq_k, num_heads, head_dim, dtype);
+  FlashParams f{};
+  f.batch = batch;
+  f.seq_q = seq_q;
+  f.seq_k = seq_k;
+  f.heads = num_heads;
+  const int64_t splits = flash_window_splits(window_params(f, w), (int)head_dim, dtype == CA_BF16);
+  return splits > 1 ? batch * num_heads * seq_q * splits * (head_dim + 2) * 4 : 0;
+}
+
+extern "C" int ca_flash_window(const ca_flash_window_args* wa, void* stream) {
+  if (!wa) return CA_DECLINED;
+  const ca_flash_args* a = &wa->flash;
+  if (!dtype_ok(a->dtype) || !head_dim_ok(a->head_dim) || wa->sinks < 0 || !scale_ok(a->scale)) return CA_DECLINED;
+  if (a->batch < 0 || a->num_heads <= 0 || a->seq_q < 1 || a->seq_k < 1) return CA_DECLINED;
+  if (a->seq_q >= (1 << 30) || a->seq_k >= (1 << 30)) return CA_DECLINED;
+  const WindowSides w = window_sides(a->seq_q, a->seq_k, a->causal != 0, wa->left, wa->right, wa->sinks);
+  if (w.plain) {
+    ca_flash_args f = *a;
+    f.causal = w.causal ? 1 : 0;
+    return ca_flash(&f, stream);
+  }
+  if (a->batch == 0) return CA_OK;
+  if (!a->q || !a->k || !a->v || !a->out) return CA_DECLINED;
+  if (!aligned16(a->q) || !aligned16(a->k) || !aligned16(a->v) || !aligned16(a->out)) return CA_DECLINED;
+  for (int i = 0; i < 3; ++i)
+    if (!stride16(a->q_strides[i], a->dtype) || !stride16(a->k_strides[i], a->dtype) || !stride16(a->v_strides[i], a->dtype))
+      return CA_DECLINED;
+  FlashParams f{};
+  f.q = a->q;
+  f.k = a->k;
+  f.v = a->v;
+  f.out = a->out;
+  f.batch = a->batch;
+  f.seq_q = a->seq_q;
+  f.seq_k = a->seq_k;
+  f.heads = a->num_heads;
+  for (int i = 0; i < 3; ++i) {
+    f.qs[i] = a->q_strides[i];
+    f.ks[i] = a->k_strides[i];
+    f.vs[i] = a->v_strides[i];
+  }
+  f.c = a->scale * kLog2e;
+  WindowParams p = window_params(f, w);
+  const int64_t splits = flash_window_splits(p, (int)a->head_dim, a->dtype == CA_BF16);
+  if (splits > 1) {
+    const int64_t slots = a->batch * a->num_heads * a->seq_q * splits;
+    if (!a->workspace || !aligned16(a->workspace) || a->workspace_bytes < slots * (a->head_dim + 2) * 4) return CA_DECLINED;
+    p.part_acc = static_cast<float*>(a->workspace);
+    p.part_ml = p.part_acc + slots * a->head_dim;
+    p.workspace_bytes = a->workspace_bytes;
+  }
+  hipStream_t st = static_cast<hipStream_t>(stream);
+  return a->dtype == CA_BF16 ? flash_window_bf16_launch(p, (int)a->head_dim, st)
+                             : flash_window_f32_launch(p, (int)a->head_dim, st);
+}
+
+static int64_t win_left(int64_t left, int64_t cap) { return left < 0 || left >= cap ? -1 : left; }
+
+static int64_t win_decode_ws_bytes(int64_t slots, int64_t head_dim) { return decode_acc_bytes(slots, head_dim) + slots * 8; }
+
+extern "C" int64_t ca_decode_window_workspace_bytes(int64_t num_seqs, int64_t num_heads, int64_t head_dim,
+                                                    int64_t page_size, int64_t page_table_width, int64_t left,
+                                                    int64_t sinks) {
+  if (num_seqs < 0 || num_heads < 0 || page_size <= 0 || page_table_width < 0 || sinks < 0) return -1;
+  const int64_t cap = page_table_width * page_size;
+  const int64_t tiles = win_decode_tiles(page_table_width, page_size, win_left(left, cap), sinks < cap ? sinks : cap);
+  return win_decode_ws_bytes(win_decode_slots(num_seqs * num_heads, tiles), head_dim);
+}
+
+extern "C" int ca_decode_window(const ca_decode_window_args* wa, void* stream) {
+  if (!wa) return CA_DECLINED;
+  const ca_decode_args* a = &wa->decode;
+  if (!dtype_ok(a->dtype) || !head_dim_ok(a->head_dim) || !page_ok(a->page_size) || wa->sinks < 0 || !scale_ok(a->scale))
+    return CA_DECLINED;
+  if (a->num_seqs < 0 || a->num_heads <= 0 || a->num_blocks < 0 || a->page_table_width < 0) return CA_DECLINED;
+  if ((wa->k_scale == nullptr) != (wa->v_scale == nullptr) || a->slots) return CA_DECLINED;
+  if ((a->k_new == nullptr) != (a->v_new == nullptr) || a->new_tokens < 0 || a->new_tokens > (1 << 30)) return CA_DECLINED;
+  if (a->num_seqs == 0) return CA_OK;
+  // An empty page table or cache is never read: its pointer may be null.
+  if (!a->q || !a->lens || !a->out || (a->page_table_width > 0 && !a->page_table) ||
+      (a->num_blocks > 0 && (!a->k_cache || !a->v_cache)))
+    return CA_DECLINED;
+  if (!aligned16(a->q) || !aligned16(a->k_cache) || !aligned16(a->v_cache) || !aligned16(a->out) ||
+      !stride16(a->q_stride, a->dtype))
+    return CA_DECLINED;
+  if (a->k_new && (!aligned16(a->k_new) || !aligned16(a->v_new) || !stride16(a->kv_stride, a->dtype))) return CA_DECLINED;
+  const bool f8 = wa->k_scale != nullptr;
+  const int64_t rows = a->num_seqs * a->num_heads, cap = a->page_table_width * a->page_size;
+  const int64_t per_seq = a->new_tokens > 1 ? a->new_tokens : 1;
+  WinDecodeParams p{};
+  p.left = win_left(wa->left, cap);
+  p.sinks = wa->sinks < cap ? wa->sinks : cap;
+  const int64_t tiles = win_decode_tiles(a->page_table_width, a->page_size, p.left, p.sinks);
+  if (tiles > 0x7fffffff) return CA_DECLINED;
+  p.tiles = (int)tiles;
+  p.slots = win_decode_slots(rows, p.tiles);
+  if (p.slots > 0 && (!a->workspace || !aligned16(a->workspace) ||
+                      a->workspace_bytes < win_decode_ws_bytes(p.slots, a->head_dim)))
+    return CA_DECLINED;
+  hipStream_t st = static_cast<hipStream_t>(stream);
+  // The new tokens go in first, by a kernel of their own.
+  if (a->k_new) {
+    int r;
+    if (f8) {
+      Store8Params sp{};
+      sp.key = a->k_new;
+      sp.value = a->v_new;
+      sp.tok_stride = a->kv_stride;
+      sp.kc = static_cast<uint32_t*>(a->k_cache);
+      sp.vc = static_cast<uint32_t*>(a->v_cache);
+      sp.k_scale = wa->k_scale;
+      sp.v_scale = wa->v_scale;
+      sp.lens = a->lens;
+      sp.page_table = a->page_table;
+      sp.pt_width = a->page_table_width;
+      sp.ntok = a->num_seqs * per_seq;
+      sp.per_seq = per_seq;
+      sp.heads = a->num_heads;
+      sp.page = a->page_size;
+      sp.nblocks = a->num_blocks;
+      r = store8_launch(sp, (int)a->head_dim, a->dtype == CA_BF16, st);
+    } else {
+      const int64_t words = a->head_dim * esize(a->dtype) / 4;
+      StoreParams sp{};
+      sp.key = static_cast<const uint32_t*>(a->k_new);
+      sp.value = static_cast<const uint32_t*>(a->v_new);
+      sp.tok_stride_w = a->kv_stride * esize(a->dtype) / 4;
+      sp.kc = static_cast<uint32_t*>(a->k_cache);
+      sp.vc = static_cast<uint32_t*>(a->v_cache);
+      sp.lens = a->lens;
+      sp.page_table = a->page_table;
+      sp.pt_width = a->page_table_width;
+      sp.ntok = a->num_seqs * per_seq;
+      sp.per_seq = per_seq;
+      sp.heads = a->num_heads;
+      sp.page = a->page_size;
+      sp.nblocks = a->num_blocks;
+      r = per_seq == 1 ? store_scatter_launch(sp, (int)words, st) : store_launch(sp, (int)words, st);
+    }
+    if (r != CA_OK) return r;
+  }
+  p.q = a->q;
+  p.q_stride = a->q_stride;
+  p.kc = static_cast<const uint32_t*>(a->k_cache);
+  p.vc = a->v_cache;
+  p.lens = a->lens;
+  p.len_add = a->k_new ? (int32_t)per_seq : 0;
+  p.page_table = a->page_table;
+  p.pt_width = a->page_table_width;
+  p.heads = a->num_heads;
+  p.page = a->page_size;
+  p.nblocks = a->num_blocks;
+  p.nseqs = a->num_seqs;
+  p.c = a->scale * kLog2e;
+  p.part_acc = static_cast<float*>(a->workspace);
+  p.part_ml = reinterpret_cast<float*>(static_cast<char*>(a->workspace) + decode_acc_bytes(p.slots, a->head_dim));
+  p.out = a->out;
+  p.k_scale = wa->k_scale;
+  p.v_scale = wa->v_scale;
+  return win_decode_launch(p, (int)a->head_dim, a->dtype == CA_BF16, st);
+}
+
+extern "C" int64_t ca_store_fp8_workspace_bytes(int64_t num_tokens, int64_t num_blocks, int64_t page_size) {
+  if (num_tokens < 0 || num_blocks < 0 || page_size <= 0) return -1;
+  return store8_work_ints(num_tokens, num_blocks, page_size) * 4;
+}
+
+extern "C" int ca_store_fp8(const ca_store_fp8_args* sa, void* stream) {
+  if (!sa) return CA_DECLINED;
+  const ca_store_args* a = &sa->store;
+  if (!dtype_ok(a->dtype) || !head_dim_ok(a->head_dim) || !page_ok(a->page_size)) return CA_DECLINED;
+  if (a->num_tokens < 0 || a->num_heads <= 0 || a->num_blocks < 0) return CA_DECLINED;
+  if (a->num_tokens == 0) return CA_OK;
+  if (!a->key || !a->value || !a->k_cache || !a->v_cache || !a->slot_mapping || !sa->k_scale || !sa->v_scale)
+    return CA_DECLINED;
+  if (!aligned16(a->key) || !aligned16(a->value) || !aligned16(a->k_cache) || !aligned16(a->v_cache)) return CA_DECLINED;
+  const bool one = a->num_tokens == 1;  // its stride is not read
+  if (!one && (!stride16(a->token_stride, a->dtype) || a->token_stride < a->num_heads * a->head_dim)) return CA_DECLINED;
+  const int64_t need = ca_store_fp8_workspace_bytes(a->num_tokens, a->num_blocks, a->page_size);
+  if (need > 0 && (!sa->workspace || !aligned16(sa->workspace) || sa->workspace_bytes < need)) return CA_DECLINED;
+  Store8Params p{};
+  p.key = a->key;
+  p.value = a->value;
+  p.tok_stride = one ? 0 : a->token_stride;
+  p.kc = static_cast<uint32_t*>(a->k_cache);
+  p.vc = static_cast<uint32_t*>(a->v_cache);
+  p.k_scale = sa->k_scale;
+  p.v_scale = sa->v_scale;
+  p.slots = a->slot_mapping;
+  p.ntok = a->num_tokens;
+  p.per_seq = 1;
+  p.heads = a->num_heads;
+  p.page = a->page_size;
+  p.nblocks = a->num_blocks;
+  p.work = static_cast<int32_t*>(sa->workspace);
+  return store8_launch(p, (int)a->head_dim, a->dtype == CA_BF16, static_cast<hipStream_t>(stream));
+}
+
+extern "C" int ca_copy_blocks(const ca_copy_blocks_args* a, void* stream) {
+  if (!a || a->num_arrays < 0 || a->num_pairs < 0 || a->num_blocks < 0 || a->block_bytes <= 0 || a->block_bytes % 4)
+    return CA_DECLINED;
+  if (a->num_arrays == 0 || a->num_pairs == 0) return CA_OK;
+  if (!a->arrays || !a->mapping) return CA_DECLINED;
+  for (int64_t i = 0; i < a->num_arrays; ++i)
+    if (!a->arrays[i] || ((uintptr_t)a->arrays[i] & (a->block_bytes % 16 ? 3 : 15))) return CA_DECLINED;
+  CopyParams p{};
+  p.mapping = a->mapping;
+  p.pairs = a->num_pairs;
+  p.nblocks = a->num_blocks;
+  p.bytes = a->block_bytes;
+  for (int64_t i = 0; i < a->num_arrays; i += kCopyArrays) {
+    const int64_t left = a->num_arrays - i;
+    p.arrays = (int)(left < kCopyArrays ? left : kCopyArrays);
+    for (int k = 0; k < p.arrays; ++k) p.base[k] = a->arrays[i + k];
+    const int r = copy_launch(p, static_cast<hipStream_t>(stream));
+    if (r != CA_OK) return r;
+  }
+  return CA_OK;
+}

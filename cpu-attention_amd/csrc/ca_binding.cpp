@@ -18,12 +18,14 @@
 #include <Python.h>
 
 #include <ATen/core/Tensor.h>
+#include <c10/core/DeviceGuard.h>
 #include <ATen/ops/empty.h>
 #include <ATen/ops/max.h>
 #include <torch/csrc/Exceptions.h>
 #include <torch/csrc/autograd/python_variable.h>
 
 #include <cmath>
+#include <vector>
 
 #include "cpu_attention_hip.h"
 
@@ -36,7 +38,16 @@ struct Entries {
   int64_t (*decode_ws)(int64_t, int64_t, int64_t, int64_t, int64_t) = nullptr;
   int64_t (*flash_ws)(int64_t, int64_t, int64_t, int64_t, int64_t, int32_t) = nullptr;
   const char* (*status)(int) = nullptr;
+  int (*flash_window)(const ca_flash_window_args*, void*) = nullptr;
+  int64_t (*flash_window_ws)(int64_t, int64_t, int64_t, int64_t, int64_t, int32_t, int32_t, int64_t, int64_t,
+                             int64_t) = nullptr;
+  int (*decode_window)(const ca_decode_window_args*, void*) = nullptr;
+  int64_t (*decode_window_ws)(int64_t, int64_t, int64_t, int64_t, int64_t, int64_t, int64_t) = nullptr;
+  int (*store_fp8)(const ca_store_fp8_args*, void*) = nullptr;
+  int64_t (*store_fp8_ws)(int64_t, int64_t, int64_t) = nullptr;
+  int (*copy_blocks)(const ca_copy_blocks_args*, void*) = nullptr;
 };
+constexpr int kEntries = 13;
 
 Entries g_lib;
 PyObject* g_plain[2] = {nullptr, nullptr};  // torch.Tensor, torch.nn.Parameter
@@ -138,15 +149,18 @@ PyObject* failed(int rc, const char* what) {
 
 // init(entries, plain_types, raw_stream, host_checks): `entries` holds the
 // addresses of ca_decode, ca_store, ca_flash, ca_decode_workspace_bytes,
-// ca_flash_workspace_bytes and ca_status_string.
+// ca_flash_workspace_bytes, ca_status_string, ca_flash_window,
+// ca_flash_window_workspace_bytes, ca_decode_window,
+// ca_decode_window_workspace_bytes, ca_store_fp8, ca_store_fp8_workspace_bytes and
+// ca_copy_blocks.
 static PyObject* b_init(PyObject*, PyObject* const* args, Py_ssize_t n) {
-  if (n != 4 || !PyTuple_Check(args[0]) || PyTuple_GET_SIZE(args[0]) != 6 || !PyTuple_Check(args[1]) ||
+  if (n != 4 || !PyTuple_Check(args[0]) || PyTuple_GET_SIZE(args[0]) != kEntries || !PyTuple_Check(args[1]) ||
       PyTuple_GET_SIZE(args[1]) != 2 || !PyCallable_Check(args[2])) {
-    PyErr_SetString(PyExc_TypeError, "init(entries[6], plain_types[2], raw_stream, host_checks)");
+    PyErr_SetString(PyExc_TypeError, "init(entries[13], plain_types[2], raw_stream, host_checks)");
     return nullptr;
   }
-  void* p[6];
-  for (int i = 0; i < 6; ++i) {
+  void* p[kEntries];
+  for (int i = 0; i < kEntries; ++i) {
     p[i] = PyLong_AsVoidPtr(PyTuple_GET_ITEM(args[0], i));
     if (PyErr_Occurred()) return nullptr;
     if (!p[i]) {
@@ -160,6 +174,13 @@ static PyObject* b_init(PyObject*, PyObject* const* args, Py_ssize_t n) {
   g_lib.decode_ws = reinterpret_cast<int64_t (*)(int64_t, int64_t, int64_t, int64_t, int64_t)>(p[3]);
   g_lib.flash_ws = reinterpret_cast<int64_t (*)(int64_t, int64_t, int64_t, int64_t, int64_t, int32_t)>(p[4]);
   g_lib.status = reinterpret_cast<const char* (*)(int)>(p[5]);
+  g_lib.flash_window = reinterpret_cast<decltype(g_lib.flash_window)>(p[6]);
+  g_lib.flash_window_ws = reinterpret_cast<decltype(g_lib.flash_window_ws)>(p[7]);
+  g_lib.decode_window = reinterpret_cast<decltype(g_lib.decode_window)>(p[8]);
+  g_lib.decode_window_ws = reinterpret_cast<decltype(g_lib.decode_window_ws)>(p[9]);
+  g_lib.store_fp8 = reinterpret_cast<decltype(g_lib.store_fp8)>(p[10]);
+  g_lib.store_fp8_ws = reinterpret_cast<decltype(g_lib.store_fp8_ws)>(p[11]);
+  g_lib.copy_blocks = reinterpret_cast<decltype(g_lib.copy_blocks)>(p[12]);
   for (int i = 0; i < 2; ++i) {
     Py_XDECREF(g_plain[i]);
     g_plain[i] = PyTuple_GET_ITEM(args[1], i);
@@ -424,12 +445,297 @@ static PyObject* b_flash(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
   END_HANDLE_TH_ERRORS
 }
 
+// An 8-bit cache's scales: fp32 [blocks, heads], contiguous, two tensors.
+static bool scales_ok(PyObject* kso, PyObject* vso, const at::Tensor& kc) {
+  if (!plain(kso) || !plain(vso)) return false;
+  const at::Tensor& ks = T(kso);
+  const at::Tensor& vs = T(vso);
+  for (const at::Tensor* t : {&ks, &vs})
+    if (t->dim() != 2 || t->scalar_type() != at::kFloat || t->size(0) != kc.size(0) || t->size(1) != kc.size(1) ||
+        !t->is_contiguous() || !on_gpu(kc.device(), *t))
+      return false;
+  return ks.numel() == 0 || ks.data_ptr() != vs.data_ptr();
+}
+
+static bool to_int64(PyObject* o, int64_t* out) {
+  *out = PyLong_AsLongLong(o);
+  return !(*out == -1 && PyErr_Occurred());
+}
+
+// flash_window(rt, q, k, v, scale, causal, left, right, sinks): flash_attn_window_func over
+// q/k/v as `flash` takes them.  Returns the output, or None.
+static PyObject* b_flash_window(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
+  HANDLE_TH_ERRORS
+  if (nargs != 9) {
+    PyErr_SetString(PyExc_TypeError, "flash_window takes 9 positional arguments");
+    return nullptr;
+  }
+  if (!ready()) return nullptr;
+  PyObject *qo = args[1], *ko = args[2], *vo = args[3], *scale = args[4], *causal = args[5];
+  int64_t left, right, sinks;
+  if (!to_int64(args[6], &left) || !to_int64(args[7], &right) || !to_int64(args[8], &sinks)) return nullptr;
+  if (!(plain(qo) && plain(ko) && plain(vo))) Py_RETURN_NONE;
+  const at::Tensor& q = T(qo);
+  const at::Tensor& k = T(ko);
+  const at::Tensor& v = T(vo);
+  if (q.dim() != 4 || k.dim() != 4 || v.sizes() != k.sizes()) Py_RETURN_NONE;
+  const int64_t b = q.size(0), sq = q.size(1), heads = q.size(2), hd = q.size(3), sk = k.size(1);
+  const at::ScalarType dt = q.scalar_type();
+  if (!is_dtype(dt) || !is_hd(hd) || sq < 1 || sk < 1) Py_RETURN_NONE;
+  if (k.size(0) != b || k.size(2) != heads || k.size(3) != hd || k.scalar_type() != dt || v.scalar_type() != dt)
+    Py_RETURN_NONE;
+  if (q.stride(3) != 1 || k.stride(3) != 1 || v.stride(3) != 1) Py_RETURN_NONE;
+  if (causal != Py_True && causal != Py_False) Py_RETURN_NONE;
+  const at::Device dev = q.device();
+  if (!q.is_cuda() || k.device() != dev || v.device() != dev) Py_RETURN_NONE;
+  ca_flash_window_args w{};
+  ca_flash_args& a = w.flash;
+  for (int i = 0; i < 3; ++i) {
+    a.q_strides[i] = stride0(q, i);
+    a.k_strides[i] = stride0(k, i);
+    a.v_strides[i] = stride0(v, i);
+  }
+  if (!scale_of(scale, hd, &a.scale)) return nullptr;
+  const c10::DeviceGuard guard(dev);
+  void* stream;
+  if (!stream_of(dev, &stream)) return nullptr;
+  a.dtype = dtype_code(dt);
+  a.causal = causal == Py_True ? 1 : 0;
+  a.workspace_bytes = g_lib.flash_window_ws(b, sq, sk, heads, hd, a.dtype, a.causal, left, right, sinks);
+  at::Tensor ws;  // held past the launch
+  if (a.workspace_bytes > 0)
+    ws = at::empty({a.workspace_bytes}, at::TensorOptions().dtype(at::kByte).device(dev));
+  at::Tensor out = at::empty(q.sizes(), at::TensorOptions().dtype(dt).device(dev));
+  a.q = q.data_ptr();
+  a.k = k.data_ptr();
+  a.v = v.data_ptr();
+  a.out = out.data_ptr();
+  a.batch = b;
+  a.seq_q = sq;
+  a.seq_k = sk;
+  a.num_heads = heads;
+  a.head_dim = hd;
+  a.workspace = ws.defined() ? ws.data_ptr() : nullptr;
+  w.left = left;
+  w.right = right;
+  w.sinks = sinks;
+  const int rc = g_lib.flash_window(&w, stream);
+  if (rc == CA_DECLINED) Py_RETURN_NONE;
+  if (rc != CA_OK) return failed(rc, "flash_window");
+  return THPVariable_Wrap(std::move(out));
+  END_HANDLE_TH_ERRORS
+}
+
+// decode_window(rt, q, k_cache, v_cache, k_scale, v_scale, k, v, lens, page_table, scale,
+// left, sinks, n): paged decode of q [seqs, (1,) heads, dim] with a window and sinks, over
+// the cache of q's type (scales None) or the 8-bit one; with k/v, n new tokens per sequence
+// (rows [seqs * n, heads, dim], or q's shape for n = 1) are appended at lens first.  Returns
+// the output, or None.
+static PyObject* b_decode_window(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
+  HANDLE_TH_ERRORS
+  if (nargs != 14) {
+    PyErr_SetString(PyExc_TypeError, "decode_window takes 14 positional arguments");
+    return nullptr;
+  }
+  if (!ready()) return nullptr;
+  PyObject *qo = args[1], *kco = args[2], *vco = args[3], *kso = args[4], *vso = args[5], *ko = args[6], *vo = args[7],
+           *lo = args[8], *pto = args[9], *scale = args[10];
+  int64_t left, sinks, n;
+  if (!to_int64(args[11], &left) || !to_int64(args[12], &sinks) || !to_int64(args[13], &n)) return nullptr;
+  if (!(plain(qo) && plain(pto)) || n < 1) Py_RETURN_NONE;
+  const at::Tensor& q = T(qo);
+  const int64_t nd = q.dim();
+  if ((nd != 3 && nd != 4) || (nd == 4 && q.size(1) != 1)) Py_RETURN_NONE;
+  const int64_t b = q.size(0), heads = q.size(-2), hd = q.size(-1);
+  const at::ScalarType dt = q.scalar_type();
+  if (!is_dtype(dt) || !is_hd(hd) || !rows_ok(q, hd)) Py_RETURN_NONE;
+  const bool f8 = kso != Py_None;
+  if (!caches_ok(kco, vco, f8 ? at::kFloat8_e4m3fn : dt, heads, hd)) Py_RETURN_NONE;
+  const at::Tensor& kc = T(kco);
+  const at::Tensor& vc = T(vco);
+  const at::Tensor& pt = T(pto);
+  if (pt.dim() != 2 || pt.scalar_type() != at::kInt || pt.size(0) != b || !pt.is_contiguous()) Py_RETURN_NONE;
+  if (!int_vector(lo, at::kInt, b)) Py_RETURN_NONE;
+  const at::Device dev = q.device();
+  if (!q.is_cuda() || !on_gpu(dev, kc) || !on_gpu(dev, vc)) Py_RETURN_NONE;
+  if (f8 ? !scales_ok(kso, vso, kc) : vso != Py_None) Py_RETURN_NONE;
+  const bool store = ko != Py_None;
+  if (store) {
+    if (!(plain(ko) && plain(vo))) Py_RETURN_NONE;
+    const at::Tensor& k = T(ko);
+    const at::Tensor& v = T(vo);
+    const bool shape_ok = n == 1 ? k.sizes() == q.sizes()
+                                 : (k.dim() == 3 && k.size(0) == b * n && k.size(1) == heads && k.size(2) == hd);
+    if (!shape_ok || v.sizes() != k.sizes() || v.strides() != k.strides()) Py_RETURN_NONE;
+    if (k.scalar_type() != dt || v.scalar_type() != dt || !rows_ok(k, hd) || !on_gpu(dev, k) || !on_gpu(dev, v))
+      Py_RETURN_NONE;
+  } else if (vo != Py_None) {
+    Py_RETURN_NONE;
+  }
+  const int64_t page = kc.size(2), width = pt.size(1);
+  if (g_host_checks && b && max_of(T(lo)) + (store ? n : 0) > width * page) Py_RETURN_NONE;
+  ca_decode_window_args w{};
+  ca_decode_args& a = w.decode;
+  if (!scale_of(scale, hd, &a.scale)) return nullptr;
+  const c10::DeviceGuard guard(dev);
+  void* stream;
+  if (!stream_of(dev, &stream)) return nullptr;
+  const at::Tensor lens = index_on(T(lo), dev);
+  const at::Tensor table = index_on(pt, dev);
+  at::Tensor out = at::empty(q.sizes(), at::TensorOptions().dtype(dt).device(dev));
+  a.workspace_bytes = g_lib.decode_window_ws(b, heads, hd, page, width, left, sinks);
+  at::Tensor ws;  // held past the launch
+  if (a.workspace_bytes > 0)
+    ws = at::empty({a.workspace_bytes}, at::TensorOptions().dtype(at::kByte).device(dev));
+  a.q = q.data_ptr();
+  a.q_stride = stride0(q, 0);
+  a.k_cache = kc.data_ptr();
+  a.v_cache = vc.data_ptr();
+  a.k_new = store ? T(ko).data_ptr() : nullptr;
+  a.v_new = store ? T(vo).data_ptr() : nullptr;
+  a.kv_stride = store ? stride0(T(ko), 0) : 0;
+  a.lens = lens.data_ptr<int32_t>();
+  a.page_table = table.data_ptr<int32_t>();
+  a.page_table_width = width;
+  a.out = out.data_ptr();
+  a.num_seqs = b;
+  a.num_heads = heads;
+  a.head_dim = hd;
+  a.page_size = page;
+  a.num_blocks = kc.size(0);
+  a.dtype = dtype_code(dt);
+  a.workspace = ws.defined() ? ws.data_ptr() : nullptr;
+  a.new_tokens = store ? n : 0;
+  w.k_scale = f8 ? T(kso).data_ptr<float>() : nullptr;
+  w.v_scale = f8 ? T(vso).data_ptr<float>() : nullptr;
+  w.left = left;
+  w.sinks = sinks;
+  const int rc = g_lib.decode_window(&w, stream);
+  if (rc == CA_DECLINED) Py_RETURN_NONE;
+  if (rc != CA_OK) return failed(rc, "decode_window");
+  return THPVariable_Wrap(std::move(out));
+  END_HANDLE_TH_ERRORS
+}
+
+// store_fp8(rt, key, value, k_cache, v_cache, k_scale, v_scale, slots): reshape_and_cache_fp8.
+// True, or None.
+static PyObject* b_store_fp8(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
+  HANDLE_TH_ERRORS
+  if (nargs != 8) {
+    PyErr_SetString(PyExc_TypeError, "store_fp8 takes 8 positional arguments");
+    return nullptr;
+  }
+  if (!ready()) return nullptr;
+  PyObject *keyo = args[1], *valo = args[2], *kco = args[3], *vco = args[4], *kso = args[5], *vso = args[6],
+           *slo = args[7];
+  if (!(plain(keyo) && plain(valo))) Py_RETURN_NONE;
+  const at::Tensor& key = T(keyo);
+  const at::Tensor& val = T(valo);
+  if (key.dim() != 3 || val.dim() != 3) Py_RETURN_NONE;
+  const int64_t n = key.size(0), heads = key.size(1), hd = key.size(2);
+  const at::ScalarType dt = key.scalar_type();
+  if (!is_dtype(dt) || !is_hd(hd) || val.scalar_type() != dt || !rows_ok(key, hd)) Py_RETURN_NONE;
+  if (val.sizes() != key.sizes() || val.strides() != key.strides()) Py_RETURN_NONE;
+  if (!caches_ok(kco, vco, at::kFloat8_e4m3fn, heads, hd) || !int_vector(slo, at::kLong, n)) Py_RETURN_NONE;
+  const at::Tensor& kc = T(kco);
+  const at::Tensor& vc = T(vco);
+  const at::Device dev = kc.device();
+  if (!kc.is_cuda() || !on_gpu(dev, vc) || !on_gpu(dev, key) || !on_gpu(dev, val) || !scales_ok(kso, vso, kc))
+    Py_RETURN_NONE;
+  if (kc.numel() && kc.data_ptr() == vc.data_ptr()) Py_RETURN_NONE;
+  const int64_t page = kc.size(2), nblocks = kc.size(0);
+  if (g_host_checks && n && max_of(T(slo)) >= nblocks * page) Py_RETURN_NONE;
+  if (n == 0 || nblocks == 0) Py_RETURN_TRUE;
+  const c10::DeviceGuard guard(dev);
+  void* stream;
+  if (!stream_of(dev, &stream)) return nullptr;
+  const at::Tensor slots = index_on(T(slo), dev);
+  ca_store_fp8_args s{};
+  ca_store_args& a = s.store;
+  s.workspace_bytes = g_lib.store_fp8_ws(n, nblocks, page);
+  at::Tensor ws;  // held past the launch
+  if (s.workspace_bytes > 0)
+    ws = at::empty({s.workspace_bytes}, at::TensorOptions().dtype(at::kByte).device(dev));
+  a.key = key.data_ptr();
+  a.value = val.data_ptr();
+  a.token_stride = stride0(key, 0);
+  a.k_cache = kc.data_ptr();
+  a.v_cache = vc.data_ptr();
+  a.slot_mapping = slots.data_ptr<int64_t>();
+  a.num_tokens = n;
+  a.num_heads = heads;
+  a.head_dim = hd;
+  a.page_size = page;
+  a.num_blocks = nblocks;
+  a.dtype = dtype_code(dt);
+  s.k_scale = T(kso).data_ptr<float>();
+  s.v_scale = T(vso).data_ptr<float>();
+  s.workspace = ws.defined() ? ws.data_ptr() : nullptr;
+  const int rc = g_lib.store_fp8(&s, stream);
+  if (rc == CA_DECLINED) Py_RETURN_NONE;
+  if (rc != CA_OK) return failed(rc, "store_fp8");
+  Py_RETURN_TRUE;
+  END_HANDLE_TH_ERRORS
+}
+
+// copy_blocks(rt, arrays, mapping): pages mapping[i][0] -> mapping[i][1] (int64 [pairs, 2])
+// within each tensor of the list `arrays` (contiguous, the same shape and type, pages along
+// dim 0).  True, or None.
+static PyObject* b_copy_blocks(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
+  HANDLE_TH_ERRORS
+  if (nargs != 3) {
+    PyErr_SetString(PyExc_TypeError, "copy_blocks takes 3 positional arguments");
+    return nullptr;
+  }
+  if (!ready()) return nullptr;
+  if (!PyList_Check(args[1]) || !plain(args[2])) Py_RETURN_NONE;
+  const Py_ssize_t n = PyList_GET_SIZE(args[1]);
+  const at::Tensor& map = T(args[2]);
+  if (map.dim() != 2 || map.size(1) != 2 || map.scalar_type() != at::kLong || !map.is_contiguous()) Py_RETURN_NONE;
+  if (n == 0) Py_RETURN_TRUE;
+  std::vector<void*> ptrs(n);
+  for (Py_ssize_t i = 0; i < n; ++i) {
+    PyObject* o = PyList_GET_ITEM(args[1], i);
+    if (!plain(o)) Py_RETURN_NONE;
+    const at::Tensor& t = T(o);
+    const at::Tensor& first = T(PyList_GET_ITEM(args[1], 0));
+    if (t.dim() < 1 || !t.is_contiguous() || t.sizes() != first.sizes() || t.scalar_type() != first.scalar_type() ||
+        !t.is_cuda() || t.device() != first.device())
+      Py_RETURN_NONE;
+    ptrs[i] = t.data_ptr();
+  }
+  const at::Tensor& t = T(PyList_GET_ITEM(args[1], 0));
+  if (map.size(0) == 0 || t.numel() == 0) Py_RETURN_TRUE;
+  const at::Device dev = t.device();
+  const c10::DeviceGuard guard(dev);
+  void* stream;
+  if (!stream_of(dev, &stream)) return nullptr;
+  const at::Tensor mapping = index_on(map, dev);
+  ca_copy_blocks_args a{};
+  a.arrays = ptrs.data();
+  a.num_arrays = n;
+  a.block_bytes = (int64_t)t.nbytes() / t.size(0);
+  a.mapping = mapping.data_ptr<int64_t>();
+  a.num_pairs = map.size(0);
+  a.num_blocks = t.size(0);
+  const int rc = g_lib.copy_blocks(&a, stream);
+  if (rc == CA_DECLINED) Py_RETURN_NONE;
+  if (rc != CA_OK) return failed(rc, "copy_blocks");
+  Py_RETURN_TRUE;
+  END_HANDLE_TH_ERRORS
+}
+
 static PyMethodDef kMethods[] = {
     {"init", (PyCFunction)(void (*)(void))b_init, METH_FASTCALL, "Entry addresses, tensor types, stream query."},
     {"set_host_checks", b_set_host_checks, METH_O, "Check slots and lengths on the host."},
     {"decode", (PyCFunction)(void (*)(void))b_decode, METH_FASTCALL, "Paged decode (_C.mojo:87-171)."},
     {"store", (PyCFunction)(void (*)(void))b_store, METH_FASTCALL, "reshape_and_cache (_C.mojo:174-213)."},
     {"flash", (PyCFunction)(void (*)(void))b_flash, METH_FASTCALL, "Dense prefill (_C.mojo:232-316)."},
+    {"flash_window", (PyCFunction)(void (*)(void))b_flash_window, METH_FASTCALL, "Prefill with a window and sinks."},
+    {"decode_window", (PyCFunction)(void (*)(void))b_decode_window, METH_FASTCALL,
+     "Paged decode with a window and sinks, over the cache or the 8-bit one."},
+    {"store_fp8", (PyCFunction)(void (*)(void))b_store_fp8, METH_FASTCALL, "reshape_and_cache into the 8-bit cache."},
+    {"copy_blocks", (PyCFunction)(void (*)(void))b_copy_blocks, METH_FASTCALL, "Pages copied within arrays."},
     {nullptr, nullptr, 0, nullptr}};
 
 static PyModuleDef kModule = {PyModuleDef_HEAD_INIT, "_binding",

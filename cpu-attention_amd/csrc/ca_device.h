@@ -11,6 +11,7 @@ namespace ca {
 
 typedef __attribute__((ext_vector_type(4))) uint32_t u32x4;
 typedef __attribute__((ext_vector_type(2))) uint32_t u32x2;
+typedef __attribute__((ext_vector_type(2))) float f32x2;
 typedef __attribute__((ext_vector_type(4))) float f32x4;
 typedef __attribute__((ext_vector_type(16))) float f32x16;
 typedef __attribute__((ext_vector_type(8))) __bf16 bf16x8;
@@ -33,6 +34,14 @@ __device__ __forceinline__ float bf16_hi(uint32_t w) { return __uint_as_float(w 
 __device__ __forceinline__ uint32_t pack_bf16x2(float lo, float hi) {
   bf16x2 v = {static_cast<__bf16>(lo), static_cast<__bf16>(hi)};
   return __builtin_bit_cast(uint32_t, v);
+}
+
+// Two of a word's four e4m3 codes as fp32 (exact), and two fp32 values as codes (round to
+// nearest even; inf and NaN become NaN codes, and so does what rounds past 448).
+__device__ __forceinline__ f32x2 e4m3_lo(uint32_t w) { return __builtin_bit_cast(f32x2, __builtin_amdgcn_cvt_pk_f32_fp8((int)w, false)); }
+__device__ __forceinline__ f32x2 e4m3_hi(uint32_t w) { return __builtin_bit_cast(f32x2, __builtin_amdgcn_cvt_pk_f32_fp8((int)w, true)); }
+__device__ __forceinline__ uint32_t e4m3_word(float a, float b, float c, float d) {
+  return (uint32_t)__builtin_amdgcn_cvt_pk_fp8_f32(c, d, __builtin_amdgcn_cvt_pk_fp8_f32(a, b, 0, false), true);
 }
 
 __device__ __forceinline__ float wave_max(float x) {

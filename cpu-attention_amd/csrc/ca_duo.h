@@ -30,6 +30,12 @@
 // the combine kernel (few query blocks over long keys).
 // Pairs (causal): query blocks (nqb - 1 - j, j) one after the other, so every block
 // walks about the same number of tiles.
+//
+// Window calls (P = WindowParams, ca_window.h): the block's keys are a list of tiles, the
+// sinks' and the window's, each masked by the rows' own limits.  A row's first tile may
+// hold nothing that it sees, or a few sinks far above or below the window's logits, so
+// there is no fixed max to take from it: these calls run the walk with the running max.
+// Rows that come out not finite are redone key by key (win_redo_row).
 #pragma once
 
 namespace ca {
@@ -217,8 +223,9 @@ inline DuoPlan duo_plan(const FlashParams& p, int E, const FlashPlan& tiled) {
   return d;
 }
 
-template <int E, int KG, bool SPLIT>
-__global__ __launch_bounds__(256 * KG, (DuoCfg<E, KG>::WAVES)) void flash_duo_kernel(FlashParams p, int pair) {
+template <int E, int KG, bool SPLIT, class P = FlashParams>
+__global__ __launch_bounds__(256 * KG, (DuoCfg<E, KG>::WAVES)) void flash_duo_kernel(P p, int pair) {
+  constexpr bool WIN = std::is_same<P, WindowParams>::value;
   static_assert(KG == 1 || !SPLIT, "split calls have one key group");
   using C = DuoCfg<E, KG>;
   constexpr int BM = C::BM, BN = C::BN, NL = C::NL, NB = C::NB, TB = C::TB, NS = E / 16, ND = E / 32, NS2 = 2 * NS;
@@ -249,11 +256,20 @@ __global__ __launch_bounds__(256 * KG, (DuoCfg<E, KG>::WAVES)) void flash_duo_ke
     uint64_t addr;
     int rows;
     uint32_t buf;
+    int tile;  // WIN: the next tile's place in the list; addr is the (batch, head)'s first row
   } ks, vs;
+  WinTiles wt{};
   const uint32_t kbuf0 = lds0 + wv * 1024, vbuf0 = kbuf0 + NB * TB;
   auto issue = [&](Stream& x, uint32_t buf0, int stride2, const int (&off)[NL]) __attribute__((always_inline)) {
-    const i32x4 rs = {__builtin_amdgcn_readfirstlane((int)(uint32_t)x.addr),
-                      __builtin_amdgcn_readfirstlane((int)((x.addr >> 32) & 0xffff)),
+    uint64_t addr = x.addr;
+    if constexpr (WIN) {
+      const int k0 = win_key0(wt, x.tile, BN);
+      addr += (uint64_t)(uint32_t)k0 * (uint32_t)stride2;
+      x.rows = x.tile < wt.n ? S - k0 : 0;
+      x.tile += KG;
+    }
+    const i32x4 rs = {__builtin_amdgcn_readfirstlane((int)(uint32_t)addr),
+                      __builtin_amdgcn_readfirstlane((int)((addr >> 32) & 0xffff)),
                       __builtin_amdgcn_readfirstlane(tile_window<E>(x.rows, stride2)), 0x00020000};
     const uint32_t base = __builtin_amdgcn_readfirstlane(x.buf);
 #pragma unroll
@@ -262,8 +278,10 @@ __global__ __launch_bounds__(256 * KG, (DuoCfg<E, KG>::WAVES)) void flash_duo_ke
                    :
                    : "s"(base + i * 4096), "v"(off[i]), "s"(rs)
                    : "memory");
-    x.addr += (uint64_t)(uint32_t)(BN * stride2) * KG;
-    x.rows -= KG * BN;
+    if constexpr (!WIN) {
+      x.addr += (uint64_t)(uint32_t)(BN * stride2) * KG;
+      x.rows -= KG * BN;
+    }
     x.buf = x.buf == buf0 ? buf0 + TB : buf0;
   };
   auto issue_k = [&]() __attribute__((always_inline)) { issue(ks, kbuf0, 2 * ks1, koff); };
@@ -292,7 +310,16 @@ __global__ __launch_bounds__(256 * KG, (DuoCfg<E, KG>::WAVES)) void flash_duo_ke
   for (int pass = 0; pass < dw.n; ++pass) {
     if (pass > 0) __syncthreads();  // every wave is done with the staging of the pass before
     const int q0 = (int)(pass == 0 ? dw.qb0 : dw.qb1) * BM, r0 = q0 + 32 * wv;
-    const DuoKeys kr = duo_keys(p, q0, r0, SPLIT, SPLIT ? (int)blockIdx.y : 0, SPLIT ? (int)gridDim.y : 1, KG, grp);
+    DuoKeys kr;
+    int t0 = 0;  // WIN: the block's first tile of the list (the split mode's share)
+    if constexpr (WIN) {
+      wt = win_tiles(p, q0, BM, BN);
+      const WinRounds wr = win_rounds(p, wt, BN, r0, SPLIT ? (int)blockIdx.y : 0, SPLIT ? (int)gridDim.y : 1, KG, grp);
+      t0 = wr.t0;
+      kr = DuoKeys{0, 0, wr.nkt, wr.nkt_w};
+    } else {
+      kr = duo_keys(p, q0, r0, SPLIT, SPLIT ? (int)blockIdx.y : 0, SPLIT ? (int)gridDim.y : 1, KG, grp);
+    }
     const int kbeg = kr.kbeg, nkt = kr.nkt, nkt_w = kr.nkt_w;
 
     bf16x8 qr[NS];  // Q^T as B operands: dims 16 s + 8 hf .. of row r0 + li
@@ -307,6 +334,21 @@ __global__ __launch_bounds__(256 * KG, (DuoCfg<E, KG>::WAVES)) void flash_duo_ke
 
     // -inf for the keys of tile t (of this group) past the row's limit.
     auto mask = [&](f32x16 (&sx)[2], int t) __attribute__((always_inline)) {
+      if constexpr (WIN) {
+        const int k0 = win_key0(wt, t0 + t * KG + grp, BN), pos = r0 + diag;  // the wave's first row's position
+        if (k0 + BN <= imin(S, pos + p.right + 1) && (k0 >= pos + 31 - p.left || k0 + BN <= p.sinks)) return;
+        int hi = imin(S - 1, pos + li + p.right) - k0 - 4 * hf, lo = imax(0, pos + li - p.left) - k0 - 4 * hf;
+        int sk = p.sinks - k0 - 4 * hf;
+        asm volatile("" : "+v"(hi), "+v"(lo), "+v"(sk));  // as below
+#pragma unroll
+        for (int kt = 0; kt < 2; ++kt)
+#pragma unroll
+          for (int r = 0; r < 16; ++r) {
+            const int x = 32 * kt + 8 * (r >> 2) + (r & 3);
+            sx[kt][r] = x <= hi && (x >= lo || x < sk) ? sx[kt][r] : -INFINITY;
+          }
+        return;
+      }
       const int k0 = kbeg + (t * KG + grp) * BN;
       if (k0 + BN > S || (p.causal && k0 + BN - 1 > r0 + diag)) {
         int vis = S - 1 - k0;
@@ -340,8 +382,12 @@ __global__ __launch_bounds__(256 * KG, (DuoCfg<E, KG>::WAVES)) void flash_duo_ke
       nmu = 0.f;
       l = 0.f;
       const int64_t first = kbeg + grp * BN;
-      ks = Stream{reinterpret_cast<uint64_t>(kg + first * ks1), kr.keys - grp * BN, kbuf0};
-      vs = Stream{reinterpret_cast<uint64_t>(vg + first * vs1), kr.keys - grp * BN, vbuf0};
+      ks = Stream{reinterpret_cast<uint64_t>(kg + first * ks1), kr.keys - grp * BN, kbuf0, 0};
+      vs = Stream{reinterpret_cast<uint64_t>(vg + first * vs1), kr.keys - grp * BN, vbuf0, 0};
+      if constexpr (WIN) {
+        ks = Stream{reinterpret_cast<uint64_t>(kg), 0, kbuf0, t0 + grp};
+        vs = Stream{reinterpret_cast<uint64_t>(vg), 0, vbuf0, t0 + grp};
+      }
       if (nkt > 0) {
         issue_k();
         issue_v();
@@ -465,8 +511,13 @@ __global__ __launch_bounds__(256 * KG, (DuoCfg<E, KG>::WAVES)) void flash_duo_ke
 
     // One loop body serves both walks; the block takes the second where a wave failed.
     bool safe = false;
+    if constexpr (WIN) {
+      walk(true);
+      __syncthreads();  // the tile buffers are free
+      safe = true;
+    }
 #pragma unroll 1
-    for (;;) {
+    while (!WIN) {
       const bool fine = walk(safe);
       __syncthreads();  // the tile buffers are free
       if (safe) break;
@@ -503,6 +554,45 @@ __global__ __launch_bounds__(256 * KG, (DuoCfg<E, KG>::WAVES)) void flash_duo_ke
         for (int r = 0; r < 16; ++r) o[d][r] = o[d][r] * w0 + mb[64 * (16 * d + r)] * w1;
     }
     float lt = l + __shfl_xor(l, 32);
+    // WIN: the rows (bit li) whose sums are not finite, which win_redo_row does again over
+    // the block's tiles, after the stores below.
+    uint32_t redo = 0;
+    auto redo_rows = [&]() __attribute__((always_inline)) {
+      if constexpr (WIN) {
+        if (__builtin_expect(redo == 0, 1)) return;
+        __builtin_amdgcn_fence(__ATOMIC_RELEASE, "workgroup");
+        __builtin_amdgcn_wave_barrier();
+        __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "workgroup");
+        const int chunk = SPLIT ? (wt.n + (int)gridDim.y - 1) / (int)gridDim.y : wt.n;
+        while (redo) {
+          const int row = r0 + __builtin_ctz(redo);
+          redo &= redo - 1;
+          if (row >= L) continue;
+          win_redo_row<E, uint16_t, BN>(p, wt, t0, imin(wt.n, t0 + chunk), qg, kg, vg, row,
+                                        [&](float rm, float rl, int d, float a) __attribute__((always_inline)) {
+            if constexpr (SPLIT) {
+              const int64_t slot = (((int64_t)dw.b * p.heads + dw.h) * p.seq_q + row) * gridDim.y + blockIdx.y;
+              p.part_acc[slot * E + d] = a;
+              if (d == 0) {
+                p.part_ml[2 * slot] = rm;
+                p.part_ml[2 * slot + 1] = rl;
+              }
+            } else {
+              out[(int64_t)row * p.heads * E + d] = (uint16_t)pack_bf16x2(rl != 0.f ? a / rl : 0.f, 0.f);
+            }
+          });
+        }
+      }
+    };
+    if constexpr (WIN) {
+      bool bad = !(fabsf(lt) < INFINITY);
+#pragma unroll
+      for (int d = 0; d < ND; ++d)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) bad |= !(fabsf(o[d][r]) < INFINITY);
+      const uint64_t b = __ballot(bad);
+      redo = (uint32_t)b | (uint32_t)(b >> 32);
+    }
     if constexpr (SPLIT) {
       // The rows' partials for the combine: O unnormalised, m (scaled log2 units), l.
       const float f = level_partial(m, lt);
@@ -520,6 +610,7 @@ __global__ __launch_bounds__(256 * KG, (DuoCfg<E, KG>::WAVES)) void flash_duo_ke
           p.part_ml[2 * slot + 1] = lt;
         }
       }
+      redo_rows();
       continue;
     }
     // out = O / l, staged through this wave's part of the tile buffers so that each
@@ -544,7 +635,36 @@ __global__ __launch_bounds__(256 * KG, (DuoCfg<E, KG>::WAVES)) void flash_duo_ke
       const u32x4 v = *reinterpret_cast<const u32x4*>(stage + rr * C::STAGE_ROW + ch * 16);
       if (row < L) __builtin_nontemporal_store(v, reinterpret_cast<u32x4*>(out + (int64_t)row * p.heads * E + ch * 8));
     }
+    redo_rows();
   }
+}
+
+// How a window call runs: kg key groups and the splits of its blocks' tiles (1: none).
+struct WinPlan {
+  int kg;
+  int64_t items, splits;
+};
+inline WinPlan win_plan(const WindowParams& p) {
+  constexpr int BM = DuoCfg<64, 1>::BM, BN = DuoCfg<64, 1>::BN;
+  WinPlan w{1, p.batch * p.heads * cdiv(p.seq_q, BM), 1};
+  const int64_t T = win_most_tiles(p, BM, BN);
+  if (w.items <= 64 && T >= 16) w.splits = 256 / w.items < T / 4 ? 256 / w.items : T / 4;
+  if (w.splits <= 1 && w.items <= 256 && T > 8) w.kg = 2;
+  return w;
+}
+
+template <int E>
+static int win_launch(const WindowParams& p, hipStream_t stream) {
+  using C1 = DuoCfg<E, 1>;
+  using C2 = DuoCfg<E, 2>;
+  const WinPlan w = win_plan(p);
+  if (w.splits > 1) {
+    const int st = launch_lds(flash_duo_kernel<E, 1, true, WindowParams>, w.items, 256, C1::LDS_BYTES, p, stream, w.splits, 0);
+    return st == CA_OK ? flash_combine_launch(p, E, true, w.splits, stream) : st;
+  }
+  if (w.kg == 2)
+    return launch_lds(flash_duo_kernel<E, 2, false, WindowParams>, w.items, 512, C2::LDS_BYTES, p, stream, 1, 0);
+  return launch_lds(flash_duo_kernel<E, 1, false, WindowParams>, w.items, 256, C1::LDS_BYTES, p, stream, 1, 0);
 }
 
 template <int E>

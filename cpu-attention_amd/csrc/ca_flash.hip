@@ -29,6 +29,7 @@
 
 #include "ca_device.h"
 #include "ca_internal.h"
+#include "ca_window.h"
 
 namespace ca {
 
@@ -47,9 +48,6 @@ __host__ __device__ inline int window_bytes(int64_t bytes) {
 __device__ __forceinline__ __amdgpu_buffer_rsrc_t tile_rsrc(const void* base, int64_t bytes) {
   return __builtin_amdgcn_make_buffer_rsrc(const_cast<void*>(base), (short)0, window_bytes(bytes), 0x00020000);
 }
-
-__host__ __device__ inline int imin(int a, int b) { return a < b ? a : b; }
-__host__ __device__ inline int imax(int a, int b) { return a > b ? a : b; }
 
 struct BlockWork {
   int64_t b, h, q0;
@@ -1199,8 +1197,8 @@ __global__ __launch_bounds__(256, 2) void flash_f32_exact_kernel(FlashParams p) 
   }
 }
 
-template <typename K, typename... A>
-static int launch_lds(K kernel, int64_t nb, int threads, int lds, const FlashParams& p, hipStream_t stream,
+template <typename K, typename P, typename... A>
+static int launch_lds(K kernel, int64_t nb, int threads, int lds, const P& p, hipStream_t stream,
                       int64_t ny = 1, A... args) {
   if (nb > 0x7fffffff || ny > 0xffff) return CA_DECLINED;
   if (lds > 64 * 1024) {
@@ -1311,6 +1309,18 @@ int flash_launch(const FlashParams& p, int E, int bf16, hipStream_t stream) {
       case 64: return f32_launch<64>(p, plan, stream);
       case 128: return f32_launch<128>(p, plan, stream);
     }
+  }
+  return CA_DECLINED;
+}
+
+int64_t flash_window_splits(const WindowParams& p, int E, bool bf16) { return bf16 ? win_plan(p).splits : 1; }
+
+int flash_window_bf16_launch(const WindowParams& p, int E, hipStream_t stream) {
+  if (!window_fits(p, E, 2)) return CA_DECLINED;
+  switch (E) {
+    case 32: return win_launch<32>(p, stream);
+    case 64: return win_launch<64>(p, stream);
+    case 128: return win_launch<128>(p, stream);
   }
   return CA_DECLINED;
 }

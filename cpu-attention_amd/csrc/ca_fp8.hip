@@ -1,0 +1,350 @@
+// Tokens into the 8-bit cache: e4m3 codes with one power-of-two scale per (page, head),
+// for K and for V each.
+//
+// The rule, for each page and head that a call puts tokens in.  With a the largest finite
+// magnitude among those tokens' elements of the head,
+//   need = the smallest 2^k, k >= -100, with a <= 448 * 2^k (448: e4m3's largest value);
+//   a call that writes the page's position 0 starts the page anew: scale = need, and
+//   what the page held is forgotten (its other codes stay, under a scale that is not
+//   theirs); any other call keeps what it holds: scale = max(scale, need), and if that
+//   grew, the page's codes become e4m3(code * old / scale);
+//   each token's code is e4m3(x / scale), rounded to nearest even; inf and NaN are NaN
+//   codes and take no part in a.
+// Scales are powers of two, so dividing by them is exact and a value is rounded once;
+// rescaling a code is exact too unless it becomes subnormal (below 2^-6, whose step then is
+// 2^-18 of the page's largest value).  Growing is what lets a page be filled token by
+// token without knowing what comes; pages are filled from position 0 on.
+//
+// Work split: one wave per (page, head).  It reads the head's rows of the page's tokens
+// (16 positions at a time, 8 dims per lane: the next positions' loads are all in flight),
+// takes both maxima by a wave reduction, rescales if it must, and writes V's rows as they
+// come and K's words transposed through LDS, 16 bytes (4 neighbouring tokens) at a time.
+// Nobody else touches the page's codes or scales, so nothing is atomic and the result
+// does not depend on the order of anything.
+//
+// Which tokens a page gets:
+//   append mode  (decode): positions lens[s] .. + per_seq - 1 of sequence s, by arithmetic;
+//   slot mode    (reshape_and_cache_fp8): slots in any order, of many pages.  A slot named
+//                twice takes its last token.  Up to kScanTokens tokens, each wave's block
+//                scans the slots for its page's (the block of a page's first token does the
+//                page).  Above, two kernels write each slot's last token into a table over
+//                the cache's slots and list the pages, and a fixed grid walks that list.
+//
+// Bound: reading the tokens and writing their codes (HBM); launches for a few tokens.
+#include "ca_device.h"
+#include "ca_internal.h"
+
+namespace ca {
+
+constexpr int kMinScaleExp = -100;
+constexpr float kMinScale = 0x1p-100f;
+constexpr int kStore8Waves = 4;       // heads per block
+constexpr int64_t kScanTokens = 1024;  // tokens up to which each block scans the slots
+constexpr int64_t kScanPage = 1024;    // positions of a page up to which it can
+
+// The smallest power of two from 2^-100 that takes magnitudes up to `top` (finite) to 448
+// = 1.75 * 2^8.
+__device__ __forceinline__ float scale_for(float top) {
+  const uint32_t b = __float_as_uint(top);
+  int k = (int)(b >> 23) - 127 - 8 + ((b & 0x7fffffu) > 0x600000u ? 1 : 0);
+  k = k > kMinScaleExp ? k : kMinScaleExp;
+  return __uint_as_float((uint32_t)(k + 127) << 23);
+}
+
+// The larger of a and |x|, if x is finite.
+__device__ __forceinline__ float max_finite(float a, float x) {
+  const float y = fabsf(x);
+  return fmaxf(a, y < INFINITY ? y : 0.f);
+}
+
+// Eight elements of a row at element index i.
+template <bool BF>
+__device__ __forceinline__ void load8(const void* src, int64_t i, float (&x)[8]) {
+  if constexpr (BF) {
+    const u32x4 w = __builtin_nontemporal_load(reinterpret_cast<const u32x4*>(reinterpret_cast<const uint16_t*>(src) + i));
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      const uint32_t v = w[k];
+      x[2 * k] = bf16_lo(v);
+      x[2 * k + 1] = bf16_hi(v);
+    }
+  } else {
+    const float* f = reinterpret_cast<const float*>(src) + i;
+#pragma unroll
+    for (int k = 0; k < 2; ++k) {
+      const f32x4 w = __builtin_nontemporal_load(reinterpret_cast<const f32x4*>(f + 4 * k));
+#pragma unroll
+      for (int j = 0; j < 4; ++j) x[4 * k + j] = w[j];
+    }
+  }
+}
+
+// n words of codes at `at` times `ratio`, by one wave.
+__device__ __forceinline__ void rescale(uint32_t* at, int64_t words, float ratio, int lane) {
+  for (int64_t i = 4 * lane; i < words; i += 4 * kWave) {
+    u32x4 w = *reinterpret_cast<const u32x4*>(at + i);
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      const uint32_t v = w[k];
+      const f32x2 lo = e4m3_lo(v), hi = e4m3_hi(v);
+      w[k] = e4m3_word(lo.x * ratio, lo.y * ratio, hi.x * ratio, hi.y * ratio);
+    }
+    *reinterpret_cast<u32x4*>(at + i) = w;
+  }
+}
+
+template <int E>
+struct Store8Shape {
+  static constexpr int W = E / 4;          // words per row of codes
+  static constexpr int LPR = E / 8;        // lanes per row
+  static constexpr int RPL = kWave / LPR;  // rows per load
+  static constexpr int NL = 16 / RPL;      // loads of 16 positions
+  static constexpr int LD = 20;            // LDS words per K word row (16 positions, padded)
+};
+
+// Puts the tokens of (blk, h) into the cache: token_of(t) names position t's token, or is
+// negative.  One wave; kl is its W * LD words of LDS.
+template <int E, bool BF, typename F>
+__device__ __forceinline__ void store_page(const Store8Params& p, int64_t blk, int64_t h, uint32_t* kl, F&& token_of) {
+  using D = Store8Shape<E>;
+  constexpr int W = D::W, LPR = D::LPR, RPL = D::RPL, NL = D::NL, LD = D::LD;
+  const int lane = threadIdx.x & 63, r = lane / LPR, dl = lane % LPR;
+  const int64_t bh = blk * p.heads + h;
+  uint32_t* kw = p.kc + bh * p.page * W;
+  uint32_t* vw = p.vc + bh * p.page * W;
+  float kx[NL][8], vx[NL][8];
+  int64_t tok[NL];
+  auto load = [&](int64_t t0) {
+#pragma unroll
+    for (int i = 0; i < NL; ++i) {
+      tok[i] = token_of(t0 + i * RPL + r);
+      if (tok[i] >= 0) {
+        const int64_t at = tok[i] * p.tok_stride + h * E + 8 * dl;
+        load8<BF>(p.key, at, kx[i]);
+        load8<BF>(p.value, at, vx[i]);
+      }
+    }
+  };
+  // The maxima, over every 16 positions of the page.  The last ones that hold a token stay
+  // in registers: usually all there is.
+  float mk = 0.f, mv = 0.f;
+  int64_t held = -1;
+  bool anew = false;
+  for (int64_t t0 = 0; t0 < p.page; t0 += 16) {
+    int64_t any = -1;
+#pragma unroll
+    for (int i = 0; i < NL; ++i) any = max<int64_t>(any, token_of(t0 + i * RPL + r));
+    if (!__any(any >= 0)) continue;
+    load(t0);
+    held = t0;
+    if (t0 == 0) anew = __any(r == 0 && tok[0] >= 0);
+#pragma unroll
+    for (int i = 0; i < NL; ++i)
+      if (tok[i] >= 0) {
+#pragma unroll
+        for (int x = 0; x < 8; ++x) {
+          mk = max_finite(mk, kx[i][x]);
+          mv = max_finite(mv, vx[i][x]);
+        }
+      }
+  }
+  if (held < 0) return;
+  float ks = scale_for(wave_max(mk)), vs = scale_for(wave_max(mv));
+  if (!anew) {
+    const float ko = p.k_scale[bh], vo = p.v_scale[bh];
+    const float k0 = ko >= kMinScale ? ko : kMinScale, v0 = vo >= kMinScale ? vo : kMinScale;
+    if (ks > k0) rescale(kw, p.page * W, k0 / ks, lane);
+    if (vs > v0) rescale(vw, p.page * W, v0 / vs, lane);
+    ks = fmaxf(ks, k0);
+    vs = fmaxf(vs, v0);
+    // The tokens' words go over rescaled ones that other lanes wrote.
+    __builtin_amdgcn_fence(__ATOMIC_RELEASE, "workgroup");
+    __builtin_amdgcn_wave_barrier();
+    __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "workgroup");
+  }
+  const float ki = 1.f / ks, vi = 1.f / vs;
+  for (int64_t t0 = held; t0 >= 0; t0 -= 16) {
+    if (t0 != held) {
+      int64_t any = -1;
+#pragma unroll
+      for (int i = 0; i < NL; ++i) any = max<int64_t>(any, token_of(t0 + i * RPL + r));
+      if (!__any(any >= 0)) continue;
+      load(t0);
+    }
+    uint32_t own = 0;  // positions of the 16 that get a token
+    wave_lds_sync();   // the reads of the 16 before
+#pragma unroll
+    for (int i = 0; i < NL; ++i) {
+      const uint64_t b = __ballot(tok[i] >= 0);
+#pragma unroll
+      for (int k = 0; k < RPL; ++k) own |= (uint32_t)(b >> (k * LPR) & 1) << (i * RPL + k);
+      if (tok[i] >= 0) {
+        const int t = i * RPL + r;
+        float* k = kx[i];
+        float* v = vx[i];
+        kl[(2 * dl) * LD + t] = e4m3_word(k[0] * ki, k[1] * ki, k[2] * ki, k[3] * ki);
+        kl[(2 * dl + 1) * LD + t] = e4m3_word(k[4] * ki, k[5] * ki, k[6] * ki, k[7] * ki);
+        *reinterpret_cast<u32x2*>(vw + (t0 + t) * W + 2 * dl) =
+            u32x2{e4m3_word(v[0] * vi, v[1] * vi, v[2] * vi, v[3] * vi), e4m3_word(v[4] * vi, v[5] * vi, v[6] * vi, v[7] * vi)};
+      }
+    }
+    wave_lds_sync();
+#pragma unroll
+    for (int x = lane; x < 4 * W; x += kWave) {
+      const int w = x >> 2, tq = x & 3;
+      const uint32_t mine = own >> (4 * tq) & 15u;
+      const u32x4 q = *reinterpret_cast<const u32x4*>(kl + w * LD + 4 * tq);
+      uint32_t* to = kw + w * p.page + t0 + 4 * tq;
+      if (mine == 15u) {
+        *reinterpret_cast<u32x4*>(to) = q;
+      } else {
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+          if (mine >> j & 1) to[j] = q[j];
+      }
+    }
+  }
+  if (lane == 0) {
+    p.k_scale[bh] = ks;
+    p.v_scale[bh] = vs;
+  }
+}
+
+// Append mode: block (sequence and 4 heads, k-th page from position lens[s] on).
+template <int E, bool BF>
+__global__ __launch_bounds__(64 * kStore8Waves) void store8_append_kernel(Store8Params p) {
+  __shared__ __attribute__((aligned(16))) uint32_t kl[kStore8Waves][Store8Shape<E>::W * Store8Shape<E>::LD];
+  const int wv = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int64_t hg = cdiv(p.heads, kStore8Waves);
+  const int64_t seq = blockIdx.x / hg, h = (blockIdx.x - seq * hg) * kStore8Waves + wv;
+  if (h >= p.heads) return;
+  const int64_t len = p.lens[seq], n = p.per_seq;
+  if (len < 0) return;
+  for (int64_t pi = len / p.page + blockIdx.y; pi < p.pt_width && pi * p.page < len + n; pi += gridDim.y) {
+    const int64_t blk = p.page_table[seq * p.pt_width + pi], first = pi * p.page;
+    if (blk < 0 || blk >= p.nblocks) continue;
+    store_page<E, BF>(p, blk, h, kl[wv], [&](int64_t t) -> int64_t {
+      const int64_t i = first + t - len;
+      return i >= 0 && i < n ? seq * n + i : -1;
+    });
+  }
+}
+
+// The page of slot s, or -1 for padding and slots past the cache.
+__device__ __forceinline__ int64_t slot_page(const Store8Params& p, int64_t s) {
+  return s >= 0 && s < p.nblocks * p.page ? s / p.page : -1;
+}
+
+// Slot mode, few tokens: block (token, 4 heads); the block of a page's first token does
+// the page.
+template <int E, bool BF>
+__global__ __launch_bounds__(64 * kStore8Waves) void store8_scan_kernel(Store8Params p) {
+  __shared__ __attribute__((aligned(16))) uint32_t kl[kStore8Waves][Store8Shape<E>::W * Store8Shape<E>::LD];
+  __shared__ int owner[kScanPage];
+  const int wv = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int64_t hg = cdiv(p.heads, kStore8Waves);
+  const int64_t i = blockIdx.x / hg, h = (blockIdx.x - i * hg) * kStore8Waves + wv;
+  const int64_t blk = slot_page(p, p.slots[i]);
+  if (blk < 0) return;
+  for (int t = threadIdx.x; t < p.page; t += 64 * kStore8Waves) owner[t] = -1;
+  __syncthreads();
+  bool earlier = false;
+  for (int64_t j = threadIdx.x; j < p.ntok; j += 64 * kStore8Waves) {
+    const int64_t s = p.slots[j];
+    if (slot_page(p, s) == blk) {
+      earlier |= j < i;
+      atomicMax(&owner[s - blk * p.page], (int)j);
+    }
+  }
+  if (__syncthreads_or(earlier) || h >= p.heads) return;
+  store_page<E, BF>(p, blk, h, kl[wv], [&](int64_t t) -> int64_t { return owner[t]; });
+}
+
+// Slot mode, many tokens.  p.work: [slots of the cache] each slot's last token, [blocks]
+// whether a page is listed, the number of pages listed, the pages; all -1 at first (the
+// number counts from -1).
+__device__ __forceinline__ int32_t* work_listed(const Store8Params& p) { return p.work + p.nblocks * p.page; }
+__device__ __forceinline__ int32_t* work_count(const Store8Params& p) { return work_listed(p) + p.nblocks; }
+
+__global__ __launch_bounds__(256) void store8_clear_kernel(int32_t* work, int64_t n) {
+  for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < n; i += (int64_t)gridDim.x * 256) work[i] = -1;
+}
+
+__global__ __launch_bounds__(256) void store8_list_kernel(Store8Params p) {
+  const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
+  if (i >= p.ntok) return;
+  const int64_t s = p.slots[i], blk = slot_page(p, s);
+  if (blk < 0) return;
+  atomicMax(p.work + s, (int)i);
+  if (atomicExch(work_listed(p) + blk, 0) == -1) {
+    int32_t* count = work_count(p);
+    count[2 + atomicAdd(count, 1)] = (int)blk;
+  }
+}
+
+template <int E, bool BF>
+__global__ __launch_bounds__(64 * kStore8Waves) void store8_pages_kernel(Store8Params p) {
+  __shared__ __attribute__((aligned(16))) uint32_t kl[kStore8Waves][Store8Shape<E>::W * Store8Shape<E>::LD];
+  const int wv = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int64_t hg = cdiv(p.heads, kStore8Waves);
+  const int32_t* count = work_count(p);
+  const int64_t units = ((int64_t)count[0] + 1) * hg;
+  for (int64_t u = blockIdx.x; u < units; u += gridDim.x) {
+    const int64_t i = u / hg, h = (u - i * hg) * kStore8Waves + wv;
+    if (h >= p.heads) continue;
+    const int64_t blk = count[1 + i];
+    const int32_t* owner = p.work + blk * p.page;
+    store_page<E, BF>(p, blk, h, kl[wv], [&](int64_t t) -> int64_t { return owner[t]; });
+  }
+}
+
+int64_t store8_work_ints(int64_t ntok, int64_t nblocks, int64_t page) {
+  if (ntok <= kScanTokens && page <= kScanPage) return 0;
+  return nblocks * page + nblocks + 1 + (ntok < nblocks ? ntok : nblocks);
+}
+
+template <int E, bool BF>
+static int store8_launch_t(const Store8Params& p, hipStream_t stream) {
+  const int64_t hg = cdiv(p.heads, kStore8Waves);
+  const dim3 block(64 * kStore8Waves);
+  if (!p.slots) {
+    const int64_t gx = p.ntok / p.per_seq * hg, gy = (p.per_seq + p.page - 2) / p.page + 1;  // pages of per_seq tokens
+    if (gx > 0x7fffffff) return CA_DECLINED;
+    hipLaunchKernelGGL((store8_append_kernel<E, BF>), dim3((unsigned)gx, (unsigned)(gy < 65535 ? gy : 65535)), block, 0, stream, p);
+    return ca_launch_status();
+  }
+  if (p.ntok > 0x7fffffff || p.nblocks > 0x7fffffff) return CA_DECLINED;
+  const int64_t ints = store8_work_ints(p.ntok, p.nblocks, p.page);
+  if (ints == 0) {
+    if (p.ntok * hg > 0x7fffffff) return CA_DECLINED;
+    hipLaunchKernelGGL((store8_scan_kernel<E, BF>), dim3((unsigned)(p.ntok * hg)), block, 0, stream, p);
+    return ca_launch_status();
+  }
+  const int64_t cb = cdiv(ints, 1024);
+  hipLaunchKernelGGL(store8_clear_kernel, dim3((unsigned)(cb < 4096 ? cb : 4096)), dim3(256), 0, stream, p.work, ints);
+  int st = ca_launch_status();
+  if (st != CA_OK) return st;
+  hipLaunchKernelGGL(store8_list_kernel, dim3((unsigned)cdiv(p.ntok, 256)), dim3(256), 0, stream, p);
+  st = ca_launch_status();
+  if (st != CA_OK) return st;
+  const int64_t most = (p.ntok < p.nblocks ? p.ntok : p.nblocks) * hg;
+  hipLaunchKernelGGL((store8_pages_kernel<E, BF>), dim3((unsigned)(most < 4096 ? most : 4096)), block, 0, stream, p);
+  return ca_launch_status();
+}
+
+template <bool BF>
+static int store8_launch_e(const Store8Params& p, int E, hipStream_t stream) {
+  switch (E) {
+    case 32: return store8_launch_t<32, BF>(p, stream);
+    case 64: return store8_launch_t<64, BF>(p, stream);
+    case 128: return store8_launch_t<128, BF>(p, stream);
+  }
+  return CA_DECLINED;
+}
+
+int store8_launch(const Store8Params& p, int E, int bf16, hipStream_t stream) {
+  if (p.ntok == 0) return CA_OK;
+  return bf16 ? store8_launch_e<true>(p, E, stream) : store8_launch_e<false>(p, E, stream);
+}
+
+}  // namespace ca

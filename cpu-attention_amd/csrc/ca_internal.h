@@ -56,6 +56,42 @@ struct DecodeParams {
   uint32_t* vc_store;
 };
 
+// The decode with a window and sinks, over the same cache or (k_scale) over one of e4m3
+// codes with a scale per (page, head).
+struct WinDecodeParams : DecodeParams {
+  int64_t left;           // keys before the newest that stay visible; < 0: all
+  int64_t sinks;          // first keys that stay visible
+  const float* k_scale;   // [nblocks, heads], nullptr: the cache holds q's type
+  const float* v_scale;
+};
+
+// Tokens into the cache of e4m3 codes (ca_fp8.hip).
+struct Store8Params {
+  const void* key;        // [T, H, E] rows, token stride tok_stride (elements)
+  const void* value;
+  int64_t tok_stride;
+  uint32_t* kc;           // per (block, head): E/4 word rows of P tokens (K transposed)
+  uint32_t* vc;           // per (block, head): P rows of E/4 words
+  float* k_scale;         // [nblocks, heads]
+  float* v_scale;
+  const int64_t* slots;   // slot mode: [T]; nullptr selects append mode
+  const int32_t* lens;    // append mode: [T / per_seq] positions
+  const int32_t* page_table;
+  int64_t pt_width;
+  int64_t ntok, heads, page, nblocks, per_seq;
+  int32_t* work;          // slot mode of many tokens: store8_work_ints() of them
+};
+
+// Pages copied within each of a list of arrays (ca_copy.hip).
+constexpr int kCopyArrays = 128;  // arrays of one launch
+struct CopyParams {
+  const int64_t* mapping;  // [pairs, 2]: source and destination page
+  int64_t pairs, nblocks;
+  int64_t bytes;           // of a page in each array
+  int arrays;
+  void* base[kCopyArrays];
+};
+
 struct FlashParams {
   const void* q;
   const void* k;
@@ -70,6 +106,13 @@ struct FlashParams {
   float* part_acc;              // [batch*heads*seq_q, splits, E]
   float* part_ml;               // [batch*heads*seq_q, splits, 2]: max (scaled log2 units), sum
   int64_t workspace_bytes;
+};
+
+// A prefill with a sliding window and sinks: row i (position i + seq_k - seq_q = pos) sees
+// keys pos - left .. pos + right, and of the first `sinks` those up to pos + right.
+// left, right and sinks lie in 0 .. 2^30 (an open side: 2^30), c > 0; `causal` is not read.
+struct WindowParams : FlashParams {
+  int32_t left, right, sinks;
 };
 
 // Calls with few query rows take the few-rows route (ca_rows.hip): up to 4 rows
@@ -248,6 +291,13 @@ int decode_tile_keys(int64_t rows, int64_t pt_width, int64_t page, int64_t head_
 int64_t decode_tiles(int64_t pt_width, int64_t page, int tile_keys);
 int64_t decode_workspace_slots(int64_t rows, int64_t tiles);
 int decode_launch(const DecodeParams& p, int head_dim, int bf16, hipStream_t stream);
+int64_t win_decode_tiles(int64_t pt_width, int64_t page, int64_t left, int64_t sinks);
+int64_t win_decode_slots(int64_t rows, int64_t tiles);
+int win_decode_launch(const WinDecodeParams& p, int head_dim, int bf16, hipStream_t stream);
+// 32-bit words of scratch that a store of these sizes needs (0: none).
+int64_t store8_work_ints(int64_t ntok, int64_t nblocks, int64_t page);
+int store8_launch(const Store8Params& p, int head_dim, int bf16, hipStream_t stream);
+int copy_launch(const CopyParams& p, hipStream_t stream);
 // ca_decode_noalloc's scratch on the current device (and that device's index),
 // and the ordering of the calls that use it: see ca_noalloc.hip.
 int decode_noalloc_scratch(void** ptr, int* device);
@@ -279,6 +329,10 @@ FlashPlan rows_plan(const FlashParams& p, int head_dim, bool bf16);
 // The short-key route's plan (small_route) and launch.
 FlashPlan small_plan(const FlashParams& p);
 int flash_small_launch(const FlashParams& p, const FlashPlan& plan, int head_dim, hipStream_t stream);
+// The prefill with a window and sinks: splits of the keys (1: no workspace), and launch.
+int64_t flash_window_splits(const WindowParams& p, int head_dim, bool bf16);
+int flash_window_bf16_launch(const WindowParams& p, int head_dim, hipStream_t stream);
+int flash_window_f32_launch(const WindowParams& p, int head_dim, hipStream_t stream);
 // Merges each row's `splits` partials (p.part_acc / p.part_ml) into p.out.
 int flash_combine_launch(const FlashParams& p, int head_dim, int bf16, int64_t splits, hipStream_t stream);
 

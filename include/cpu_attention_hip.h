@@ -220,6 +220,102 @@ int64_t ca_flash_workspace_bytes(int64_t batch, int64_t seq_q, int64_t seq_k,
                                  int64_t num_heads, int64_t head_dim, int32_t dtype);
 int ca_flash(const ca_flash_args* args, void* stream);
 
+/* ---------------------------------------------------------------------------
+ * A long-running server's cache: attention with a sliding window and sinks, an
+ * 8-bit cache, and copies of pages.  No counterparts in the reference (its window
+ * and descale arguments are refused).  Conventions, return codes and checks as above.
+ * ------------------------------------------------------------------------- */
+
+/* ca_flash with a sliding window and sinks.  Row i stands at position
+ * pos = i + seq_k - seq_q and sees the keys pos - left .. pos + right, and of the first
+ * `sinks` keys those up to pos + right.  left < 0 or right < 0: no limit on that
+ * side; flash.causal sets right to 0.  A row that sees no key is exactly 0.
+ * Values of keys that a row does not see never reach it, infinities and NaNs included.
+ * flash.scale must be positive and finite.  A window that leaves nothing out of the
+ * causal or the full call runs ca_flash itself (where a key's infinities and NaNs can
+ * reach rows of its tile that do not see it).  flash.workspace: at least ca_flash_window_workspace_bytes(...) bytes
+ * (0: none), 16-byte aligned, not initialised. */
+typedef struct ca_flash_window_args {
+  ca_flash_args flash;
+  int64_t left;
+  int64_t right;
+  int64_t sinks;
+} ca_flash_window_args;
+
+int64_t ca_flash_window_workspace_bytes(int64_t batch, int64_t seq_q, int64_t seq_k,
+                                        int64_t num_heads, int64_t head_dim, int32_t dtype,
+                                        int32_t causal, int64_t left, int64_t right, int64_t sinks);
+int ca_flash_window(const ca_flash_window_args* args, void* stream);
+
+/* ca_decode with a sliding window and sinks, over the same cache or over an 8-bit one.
+ * The newest of a sequence's len tokens (after the append) sees the keys
+ * len - 1 - left .. len - 1 (left < 0: all of them) and the first `sinks` keys.
+ *
+ * k_scale == v_scale == NULL: the caches are ca_decode's.  Otherwise they hold e4m3
+ * (OCP, no infinities) codes of value / scale, with one fp32 scale per (block, head) in
+ * k_scale and v_scale, contiguous [num_blocks, num_heads]; the layout is the caches' own,
+ * a 32-bit K word holding 4 neighbouring dims: word (d / 4) * P + t.  q, out, k_new and
+ * v_new are of decode.dtype either way.  An append to an 8-bit cache follows
+ * ca_store_fp8's rule, and sequences of one call must not share the pages they
+ * append to.  decode.slots must be NULL.  decode.scale must be positive and finite.
+ * decode.workspace: at least ca_decode_window_workspace_bytes(...) bytes (0: none),
+ * 16-byte aligned, not initialised; calls that overlap must not share it. */
+typedef struct ca_decode_window_args {
+  ca_decode_args decode;
+  float* k_scale;
+  float* v_scale;
+  int64_t left;
+  int64_t sinks;
+} ca_decode_window_args;
+
+int64_t ca_decode_window_workspace_bytes(int64_t num_seqs, int64_t num_heads, int64_t head_dim,
+                                         int64_t page_size, int64_t page_table_width,
+                                         int64_t left, int64_t sinks);
+int ca_decode_window(const ca_decode_window_args* args, void* stream);
+
+/* reshape_and_cache into an 8-bit cache.  store: as for ca_store, with the caches of
+ * e4m3 codes; dtype is that of key and value.  For each page and head that the call
+ * puts tokens in, with a the largest finite magnitude of their elements and need the
+ * smallest 2^k, k >= -100, with a <= 448 * 2^k:
+ *   - a call that writes the page's position 0 starts the page anew: scale = need; the
+ *     codes of positions that the call does not write lose their meaning;
+ *   - any other call keeps the page: scale = max(scale, need) (a scale below 2^-100
+ *     counts as 2^-100), and if it grew, the page's codes are requantised:
+ *     code = e4m3(code * old / scale);
+ *   - a token's codes are e4m3(x / scale), rounded to nearest even; infinities and NaNs
+ *     become NaN codes.
+ * Scales are powers of two, so the divisions are exact.  A slot named twice takes its
+ * last token.  workspace: at least ca_store_fp8_workspace_bytes(...) bytes (0: none),
+ * 16-byte aligned, not initialised; calls that overlap must not share it. */
+typedef struct ca_store_fp8_args {
+  ca_store_args store;
+  float* k_scale; /* [num_blocks, num_heads] */
+  float* v_scale;
+  void* workspace;
+  int64_t workspace_bytes;
+} ca_store_fp8_args;
+
+int64_t ca_store_fp8_workspace_bytes(int64_t num_tokens, int64_t num_blocks, int64_t page_size);
+int ca_store_fp8(const ca_store_fp8_args* args, void* stream);
+
+/* Pages copied within each of `num_arrays` arrays of num_blocks pages of block_bytes
+ * bytes (a multiple of 4; 16-byte aligned if a multiple of 16): for pair i of mapping (device, [num_pairs, 2]),
+ * page mapping[2i] to page mapping[2i + 1].  `arrays` is a host array of device
+ * pointers, read before the call returns.  A pair with a negative page, or of a page with itself,
+ * copies nothing, and so does one past num_blocks.  Destinations must be distinct and
+ * no page both a source and a destination of two pairs: such pages end up with
+ * unspecified bytes. */
+typedef struct ca_copy_blocks_args {
+  void* const* arrays;
+  int64_t num_arrays;
+  int64_t block_bytes;
+  const int64_t* mapping;
+  int64_t num_pairs;
+  int64_t num_blocks;
+} ca_copy_blocks_args;
+
+int ca_copy_blocks(const ca_copy_blocks_args* args, void* stream);
+
 /* ABI version (CA_ABI_VERSION), a build description, and a readable status. */
 int ca_abi_version(void);
 const char* ca_version(void);

@@ -14,6 +14,8 @@ Contents (each function cites the reference file:line it restates):
   gather back to dense K/V, and paged decode on top of ``attention``:
   ``cpu_attention/_mojo/src/paged_attn.mojo:58-204, 714-782``.
 * ``bf16`` -- fp32 <-> bf16 bit conversions (round to nearest even).
+* ``serving`` -- a sliding window with sinks, the 8-bit cache and copies of pages
+  (no counterpart in the reference).
 * ``cport`` -- ctypes access to ``ca_oracle.c``: an fp32 C port of the
   reference's CPU algorithms (paged decode with base-2 online softmax over
   key steps, blocked prefill, the store), parallelised with OpenMP; used as the
