@@ -57,27 +57,23 @@ __device__ __forceinline__ float max_finite(float a, float x) {
   return fmaxf(a, y < INFINITY ? y : 0.f);
 }
 
-// Eight elements of a row at element index i.
+// Eight neighbouring elements of a row as they lie in memory, and as fp32.
 template <bool BF>
-__device__ __forceinline__ void load8(const void* src, int64_t i, float (&x)[8]) {
-  if constexpr (BF) {
-    const u32x4 w = __builtin_nontemporal_load(reinterpret_cast<const u32x4*>(reinterpret_cast<const uint16_t*>(src) + i));
+struct Row8 {
+  u32x4 w[BF ? 1 : 2];
+  __device__ __forceinline__ void load(const void* src, int64_t i) {
+    const char* at = reinterpret_cast<const char*>(src) + i * (BF ? 2 : 4);
 #pragma unroll
-    for (int k = 0; k < 4; ++k) {
-      const uint32_t v = w[k];
-      x[2 * k] = bf16_lo(v);
-      x[2 * k + 1] = bf16_hi(v);
-    }
-  } else {
-    const float* f = reinterpret_cast<const float*>(src) + i;
+    for (int k = 0; k < (BF ? 1 : 2); ++k) w[k] = __builtin_nontemporal_load(reinterpret_cast<const u32x4*>(at) + k);
+  }
+  __device__ __forceinline__ void widen(float (&x)[8]) const {
 #pragma unroll
-    for (int k = 0; k < 2; ++k) {
-      const f32x4 w = __builtin_nontemporal_load(reinterpret_cast<const f32x4*>(f + 4 * k));
-#pragma unroll
-      for (int j = 0; j < 4; ++j) x[4 * k + j] = w[j];
+    for (int k = 0; k < 8; ++k) {
+      const uint32_t v = BF ? w[0][k / 2] : w[BF ? 0 : k / 4][k % 4];
+      x[k] = !BF ? __uint_as_float(v) : (k & 1 ? bf16_hi(v) : bf16_lo(v));
     }
   }
-}
+};
 
 // n words of codes at `at` times `ratio`, by one wave.
 __device__ __forceinline__ void rescale(uint32_t* at, int64_t words, float ratio, int lane) {
@@ -112,43 +108,47 @@ __device__ __forceinline__ void store_page(const Store8Params& p, int64_t blk, i
   const int64_t bh = blk * p.heads + h;
   uint32_t* kw = p.kc + bh * p.page * W;
   uint32_t* vw = p.vc + bh * p.page * W;
-  float kx[NL][8], vx[NL][8];
-  int64_t tok[NL];
+  Row8<BF> kx[NL], vx[NL];
+  int tok[NL];
+  // The tokens of positions t0 .. t0 + 15 and their rows; whether there are any.
   auto load = [&](int64_t t0) {
+    bool any = false;
 #pragma unroll
     for (int i = 0; i < NL; ++i) {
       tok[i] = token_of(t0 + i * RPL + r);
-      if (tok[i] >= 0) {
-        const int64_t at = tok[i] * p.tok_stride + h * E + 8 * dl;
-        load8<BF>(p.key, at, kx[i]);
-        load8<BF>(p.value, at, vx[i]);
-      }
+      any |= tok[i] >= 0;
     }
-  };
-  // The maxima, over every 16 positions of the page.  The last ones that hold a token stay
-  // in registers: usually all there is.
-  float mk = 0.f, mv = 0.f;
-  int64_t held = -1;
-  bool anew = false;
-  for (int64_t t0 = 0; t0 < p.page; t0 += 16) {
-    int64_t any = -1;
+    if (!__any(any)) return false;
 #pragma unroll
-    for (int i = 0; i < NL; ++i) any = max<int64_t>(any, token_of(t0 + i * RPL + r));
-    if (!__any(any >= 0)) continue;
-    load(t0);
-    held = t0;
+    for (int i = 0; i < NL; ++i)
+      if (tok[i] >= 0) {
+        const int64_t at = (int64_t)tok[i] * p.tok_stride + h * E + 8 * dl;
+        kx[i].load(p.key, at);
+        vx[i].load(p.value, at);
+      }
+    return true;
+  };
+  // The maxima, over every 16 positions of the page.  The last ones looked at stay in
+  // registers: all there is in a page of 16, others are read again below.
+  float mk = 0.f, mv = 0.f;
+  bool found = false, anew = false;
+  for (int64_t t0 = 0; t0 < p.page; t0 += 16) {
+    if (!load(t0)) continue;
+    found = true;
     if (t0 == 0) anew = __any(r == 0 && tok[0] >= 0);
 #pragma unroll
     for (int i = 0; i < NL; ++i)
       if (tok[i] >= 0) {
+        float x[8];
+        kx[i].widen(x);
 #pragma unroll
-        for (int x = 0; x < 8; ++x) {
-          mk = max_finite(mk, kx[i][x]);
-          mv = max_finite(mv, vx[i][x]);
-        }
+        for (int j = 0; j < 8; ++j) mk = max_finite(mk, x[j]);
+        vx[i].widen(x);
+#pragma unroll
+        for (int j = 0; j < 8; ++j) mv = max_finite(mv, x[j]);
       }
   }
-  if (held < 0) return;
+  if (!found) return;
   float ks = scale_for(wave_max(mk)), vs = scale_for(wave_max(mv));
   if (!anew) {
     const float ko = p.k_scale[bh], vo = p.v_scale[bh];
@@ -163,14 +163,9 @@ __device__ __forceinline__ void store_page(const Store8Params& p, int64_t blk, i
     __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "workgroup");
   }
   const float ki = 1.f / ks, vi = 1.f / vs;
-  for (int64_t t0 = held; t0 >= 0; t0 -= 16) {
-    if (t0 != held) {
-      int64_t any = -1;
-#pragma unroll
-      for (int i = 0; i < NL; ++i) any = max<int64_t>(any, token_of(t0 + i * RPL + r));
-      if (!__any(any >= 0)) continue;
-      load(t0);
-    }
+  const int64_t last = p.page - 16;
+  for (int64_t t0 = last; t0 >= 0; t0 -= 16) {
+    if (last > 0 && !load(t0)) continue;
     uint32_t own = 0;  // positions of the 16 that get a token
     wave_lds_sync();   // the reads of the 16 before
 #pragma unroll
@@ -180,8 +175,9 @@ __device__ __forceinline__ void store_page(const Store8Params& p, int64_t blk, i
       for (int k = 0; k < RPL; ++k) own |= (uint32_t)(b >> (k * LPR) & 1) << (i * RPL + k);
       if (tok[i] >= 0) {
         const int t = i * RPL + r;
-        float* k = kx[i];
-        float* v = vx[i];
+        float k[8], v[8];
+        kx[i].widen(k);
+        vx[i].widen(v);
         kl[(2 * dl) * LD + t] = e4m3_word(k[0] * ki, k[1] * ki, k[2] * ki, k[3] * ki);
         kl[(2 * dl + 1) * LD + t] = e4m3_word(k[4] * ki, k[5] * ki, k[6] * ki, k[7] * ki);
         *reinterpret_cast<u32x2*>(vw + (t0 + t) * W + 2 * dl) =
@@ -223,9 +219,9 @@ __global__ __launch_bounds__(64 * kStore8Waves) void store8_append_kernel(Store8
   for (int64_t pi = len / p.page + blockIdx.y; pi < p.pt_width && pi * p.page < len + n; pi += gridDim.y) {
     const int64_t blk = p.page_table[seq * p.pt_width + pi], first = pi * p.page;
     if (blk < 0 || blk >= p.nblocks) continue;
-    store_page<E, BF>(p, blk, h, kl[wv], [&](int64_t t) -> int64_t {
+    store_page<E, BF>(p, blk, h, kl[wv], [&](int64_t t) -> int {
       const int64_t i = first + t - len;
-      return i >= 0 && i < n ? seq * n + i : -1;
+      return i >= 0 && i < n ? (int)(seq * n + i) : -1;
     });
   }
 }
@@ -257,7 +253,7 @@ __global__ __launch_bounds__(64 * kStore8Waves) void store8_scan_kernel(Store8Pa
     }
   }
   if (__syncthreads_or(earlier) || h >= p.heads) return;
-  store_page<E, BF>(p, blk, h, kl[wv], [&](int64_t t) -> int64_t { return owner[t]; });
+  store_page<E, BF>(p, blk, h, kl[wv], [&](int64_t t) -> int { return owner[t]; });
 }
 
 // Slot mode, many tokens.  p.work: [slots of the cache] each slot's last token, [blocks]
@@ -276,6 +272,8 @@ __global__ __launch_bounds__(256) void store8_list_kernel(Store8Params p) {
   const int64_t s = p.slots[i], blk = slot_page(p, s);
   if (blk < 0) return;
   atomicMax(p.work + s, (int)i);
+  // A run of tokens of one page asks once.
+  if (i > 0 && slot_page(p, p.slots[i - 1]) == blk) return;
   if (atomicExch(work_listed(p) + blk, 0) == -1) {
     int32_t* count = work_count(p);
     count[2 + atomicAdd(count, 1)] = (int)blk;
@@ -283,7 +281,7 @@ __global__ __launch_bounds__(256) void store8_list_kernel(Store8Params p) {
 }
 
 template <int E, bool BF>
-__global__ __launch_bounds__(64 * kStore8Waves) void store8_pages_kernel(Store8Params p) {
+__global__ __launch_bounds__(64 * kStore8Waves) __attribute__((amdgpu_waves_per_eu(5))) void store8_pages_kernel(Store8Params p) {
   __shared__ __attribute__((aligned(16))) uint32_t kl[kStore8Waves][Store8Shape<E>::W * Store8Shape<E>::LD];
   const int wv = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int64_t hg = cdiv(p.heads, kStore8Waves);
@@ -294,7 +292,7 @@ __global__ __launch_bounds__(64 * kStore8Waves) void store8_pages_kernel(Store8P
     if (h >= p.heads) continue;
     const int64_t blk = count[1 + i];
     const int32_t* owner = p.work + blk * p.page;
-    store_page<E, BF>(p, blk, h, kl[wv], [&](int64_t t) -> int64_t { return owner[t]; });
+    store_page<E, BF>(p, blk, h, kl[wv], [&](int64_t t) -> int { return owner[t]; });
   }
 }
 
@@ -307,13 +305,14 @@ template <int E, bool BF>
 static int store8_launch_t(const Store8Params& p, hipStream_t stream) {
   const int64_t hg = cdiv(p.heads, kStore8Waves);
   const dim3 block(64 * kStore8Waves);
+  if (p.ntok > 0x7fffffff) return CA_DECLINED;
   if (!p.slots) {
     const int64_t gx = p.ntok / p.per_seq * hg, gy = (p.per_seq + p.page - 2) / p.page + 1;  // pages of per_seq tokens
     if (gx > 0x7fffffff) return CA_DECLINED;
     hipLaunchKernelGGL((store8_append_kernel<E, BF>), dim3((unsigned)gx, (unsigned)(gy < 65535 ? gy : 65535)), block, 0, stream, p);
     return ca_launch_status();
   }
-  if (p.ntok > 0x7fffffff || p.nblocks > 0x7fffffff) return CA_DECLINED;
+  if (p.nblocks > 0x7fffffff) return CA_DECLINED;
   const int64_t ints = store8_work_ints(p.ntok, p.nblocks, p.page);
   if (ints == 0) {
     if (p.ntok * hg > 0x7fffffff) return CA_DECLINED;
