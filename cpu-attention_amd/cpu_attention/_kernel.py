@@ -117,8 +117,9 @@ class StoreFp8Args(ctypes.Structure):
 
 class CopyBlocksArgs(ctypes.Structure):
     """``ca_copy_blocks_args`` (include/cpu_attention_hip.h)."""
-    _fields_ = [("arrays", ctypes.POINTER(ctypes.c_void_p)), ("num_arrays", ctypes.c_int64),
-                ("block_bytes", ctypes.c_int64), ("mapping", ctypes.c_void_p),
+    _fields_ = [("caches", ctypes.POINTER(ctypes.c_void_p)), ("num_caches", ctypes.c_int64),
+                ("block_bytes", ctypes.c_int64), ("scales", ctypes.POINTER(ctypes.c_void_p)),
+                ("num_scales", ctypes.c_int64), ("row_bytes", ctypes.c_int64), ("mapping", ctypes.c_void_p),
                 ("num_pairs", ctypes.c_int64), ("num_blocks", ctypes.c_int64)]
 
 
@@ -623,28 +624,42 @@ class Module:
             self._raise(rc, "store_fp8")
         return True
 
-    def copy_blocks(self, rt, arrays, mapping):
+    def copy_blocks(self, rt, key_caches, value_caches, key_scales, value_scales, mapping):
         """Pages ``mapping[i][0]`` -> ``mapping[i][1]`` (int64 ``[pairs, 2]``) within each
-        tensor of the list ``arrays`` (contiguous, the same shape and type, pages
-        along dim 0). True, or None."""
-        if not isinstance(arrays, list) or not _plain(mapping) or mapping.dim() != 2 or mapping.shape[1] != 2 \
+        cache of the two lists (contiguous ``[blocks, heads, page, dim]`` of one shape
+        and type) and, for 8-bit caches, each scale tensor (``[blocks, heads]``; None
+        otherwise). True, or None."""
+        if not isinstance(key_caches, list) or not isinstance(value_caches, list) or not _plain(mapping) \
+                or len(key_caches) != len(value_caches) or mapping.dim() != 2 or mapping.shape[1] != 2 \
                 or mapping.dtype != torch.int64 or not mapping.is_contiguous():
             return None
-        if not arrays:
+        n, scaled = len(key_caches), key_scales is not None
+        if scaled != (value_scales is not None) or scaled and not (
+                isinstance(key_scales, list) and isinstance(value_scales, list)
+                and len(key_scales) == len(value_scales) == n):
+            return None
+        if n == 0:
             return True
-        first = arrays[0]
-        for t in arrays:
-            if not _plain(t) or t.dim() < 1 or not t.is_contiguous() or t.shape != first.shape \
-                    or t.dtype != first.dtype or not t.is_cuda or t.device != first.device:
+        first = key_caches[0]
+        if not _plain(first) or first.dtype not in (*DTYPES, FP8) or (first.dtype == FP8) != scaled \
+                or first.dim() != 4 or first.shape[3] not in HEAD_DIMS or not first.is_cuda:
+            return None
+        dev = first.device
+        for i, (k, v) in enumerate(zip(key_caches, value_caches)):
+            if not _caches_ok(k, v, first.dtype, first.shape[1], first.shape[3]) or k.shape != first.shape \
+                    or not _on_gpu(dev, k, v) or scaled and not self._scales_ok(key_scales[i], value_scales[i], k):
                 return None
+        if mapping.device != dev and mapping.device.type != "cpu":
+            return None
         if mapping.shape[0] == 0 or first.numel() == 0:
             return True
-        dev = first.device
         with torch.cuda.device(dev):
             mapping = _index_on(mapping, dev)
-            ptrs = (ctypes.c_void_p * len(arrays))(*[t.data_ptr() for t in arrays])
-            args = CopyBlocksArgs(ptrs, len(arrays), first.numel() * first.element_size() // first.shape[0],
-                                  mapping.data_ptr(), mapping.shape[0], first.shape[0])
+            caches = (ctypes.c_void_p * (2 * n))(*[t.data_ptr() for t in (*key_caches, *value_caches)])
+            scales = (ctypes.c_void_p * (2 * n))(*[t.data_ptr() for t in (*key_scales, *value_scales)]) if scaled else None
+            args = CopyBlocksArgs(caches, 2 * n, first.numel() * first.element_size() // first.shape[0], scales,
+                                  2 * n if scaled else 0, 4 * first.shape[1], mapping.data_ptr(), mapping.shape[0],
+                                  first.shape[0])
             rc = self.lib.ca_copy_blocks(ctypes.byref(args), _stream(dev))
         if rc == CA_DECLINED:
             return None

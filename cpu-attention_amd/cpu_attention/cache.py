@@ -174,39 +174,23 @@ def copy_blocks(key_caches, value_caches, block_mapping, key_scales=None, value_
     copied); with them off, such pages end up with unspecified contents, and pages past
     the caches are left out.  The copies are queued on torch's current stream.
     """
-    caches, scales = _copy_arrays(key_caches, value_caches, key_scales, value_scales)
-    if not isinstance(block_mapping, torch.Tensor) or block_mapping.dtype != torch.int64 or block_mapping.dim() != 2 \
-            or block_mapping.shape[1] != 2:
-        raise ValueError("cpu_attention: block_mapping must be int64 [num_pairs, 2]")
-    if not caches or block_mapping.shape[0] == 0:
-        return
-    dev = caches[0].device
-    if not caches[0].is_cuda or any(x.device != dev for x in caches + scales):
-        raise ValueError("cpu_attention: the MI355X build takes tensors on one ROCm GPU")
-    if any(x.data_ptr() % 16 for x in caches):
-        raise ValueError("cpu_attention: the paged caches must start 16-byte aligned")
-    if block_mapping.device.type != "cpu" and block_mapping.device != dev:
-        raise ValueError("cpu_attention: block_mapping must be on the caches' device or the CPU")
-    mapping = block_mapping.as_subclass(torch.Tensor).contiguous()
-    if K.host_checks():
-        check_mapping(mapping.cpu(), caches[0].shape[0])
-    if mapping.device != dev:
-        mapping = mapping.to(dev)
     copy, rt = K.module().copy_blocks, K.runtime()
-    for arrays in (caches, scales):
-        if copy(rt, arrays, mapping) is None:
+    if K.host_checks() or copy(rt, key_caches, value_caches, key_scales, value_scales, block_mapping) is None:
+        lists = _check_copy(key_caches, value_caches, block_mapping, key_scales, value_scales)
+        if copy(rt, *lists) is None:
             raise RuntimeError("cpu_attention: the kernel declined arguments that passed validation")
 
 
-def _copy_arrays(key_caches, value_caches, key_scales, value_scales):
-    """The caches and the scales as two lists of plain tensors, checked."""
-    keys, values = list(key_caches), list(value_caches)
+def _check_copy(key_caches, value_caches, mapping, key_scales, value_scales):
+    """Raises the error that names what is wrong with a call, or returns its arguments as
+    the kernel module takes them: lists of plain tensors, and a contiguous mapping, read
+    with host checks on."""
+    keys, values = [_plain(x) for x in key_caches], [_plain(x) for x in value_caches]
+    caches = keys + values
     if len(keys) != len(values):
         raise ValueError("cpu_attention: as many key caches as value caches")
-    caches = [x.as_subclass(torch.Tensor) for x in keys + values]
     if (key_scales is None) != (value_scales is None):
         raise ValueError("cpu_attention: pass key_scales and value_scales, or neither")
-    scales = [] if key_scales is None else [*key_scales, *value_scales]
     for x in caches:
         if x.dim() != 4 or x.shape != caches[0].shape or x.dtype != caches[0].dtype or not x.is_contiguous():
             raise ValueError("cpu_attention: the caches must be [num_blocks, nheads, page_block_size, headdim], "
@@ -217,15 +201,33 @@ def _copy_arrays(key_caches, value_caches, key_scales, value_scales):
                          "head_dim 32/64/128 and the page a multiple of 16")
     if caches and caches[0].dtype == K.FP8 and key_scales is None:
         raise ValueError("cpu_attention: 8-bit caches are copied with key_scales and value_scales")
-    if scales:
-        if caches and caches[0].dtype != K.FP8 or len(scales) != len(caches) or len(key_scales) != len(keys):
+    scales = []
+    if key_scales is not None:
+        key_scales, value_scales = ([_plain(x) for x in xs] for xs in (key_scales, value_scales))
+        scales = key_scales + value_scales
+        if caches and caches[0].dtype != K.FP8 or not len(key_scales) == len(value_scales) == len(keys):
             raise ValueError("cpu_attention: key_scales and value_scales go with 8-bit caches, one per cache")
-        for x in scales:
-            if not isinstance(x, torch.Tensor) or x.dtype != torch.float32 or x.shape != caches[0].shape[:2] \
-                    or not x.is_contiguous() or x.device != caches[0].device:
-                raise ValueError(SCALES)
-        scales = [x.as_subclass(torch.Tensor) for x in scales]
-    return caches, scales
+        for k, v, ks, vs in zip(keys, values, key_scales, value_scales):
+            check_fp8_cache(k, v, ks, vs)
+    if not isinstance(mapping, torch.Tensor) or mapping.dtype != torch.int64 or mapping.dim() != 2 or mapping.shape[1] != 2:
+        raise ValueError("cpu_attention: block_mapping must be int64 [num_pairs, 2]")
+    mapping = _plain(mapping).contiguous()
+    if caches:
+        dev = caches[0].device
+        if not caches[0].is_cuda or any(x.device != dev for x in caches + scales):
+            raise ValueError("cpu_attention: the MI355X build takes tensors on one ROCm GPU")
+        if any(x.data_ptr() % 16 for x in caches):
+            raise ValueError("cpu_attention: the paged caches must start 16-byte aligned")
+        if mapping.device.type != "cpu" and mapping.device != dev:
+            raise ValueError("cpu_attention: block_mapping must be on the caches' device or the CPU")
+        if K.host_checks():
+            check_mapping(mapping.cpu(), caches[0].shape[0])
+    return keys, values, key_scales, value_scales, mapping
+
+
+def _plain(x):
+    """Tensor subclasses become plain tensors; anything else passes through."""
+    return x.as_subclass(torch.Tensor) if isinstance(x, torch.Tensor) and type(x) is not torch.Tensor else x
 
 
 def check_mapping(mapping, num_blocks):

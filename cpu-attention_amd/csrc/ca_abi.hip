@@ -533,21 +533,25 @@ extern "C" int ca_store_fp8(const ca_store_fp8_args* sa, void* stream) {
 }
 
 extern "C" int ca_copy_blocks(const ca_copy_blocks_args* a, void* stream) {
-  if (!a || a->num_arrays < 0 || a->num_pairs < 0 || a->num_blocks < 0 || a->block_bytes <= 0 || a->block_bytes % 4)
-    return CA_DECLINED;
-  if (a->num_arrays == 0 || a->num_pairs == 0) return CA_OK;
-  if (!a->arrays || !a->mapping) return CA_DECLINED;
-  for (int64_t i = 0; i < a->num_arrays; ++i)
-    if (!a->arrays[i] || ((uintptr_t)a->arrays[i] & (a->block_bytes % 16 ? 3 : 15))) return CA_DECLINED;
+  if (!a || a->num_caches < 0 || a->num_scales < 0 || a->num_pairs < 0 || a->num_blocks < 0) return CA_DECLINED;
+  if (a->num_caches > 0 && (a->block_bytes <= 0 || a->block_bytes % 16)) return CA_DECLINED;
+  if (a->num_scales > 0 && (a->row_bytes <= 0 || a->row_bytes % 4)) return CA_DECLINED;
+  const int64_t arrays = a->num_caches + a->num_scales;
+  if (arrays == 0 || a->num_pairs == 0) return CA_OK;
+  if ((a->num_caches > 0 && !a->caches) || (a->num_scales > 0 && !a->scales) || !a->mapping) return CA_DECLINED;
+  auto array = [&](int64_t i) { return i < a->num_caches ? a->caches[i] : a->scales[i - a->num_caches]; };
+  for (int64_t i = 0; i < arrays; ++i)
+    if (!array(i) || ((uintptr_t)array(i) & (i < a->num_caches ? 15 : 3))) return CA_DECLINED;
   CopyParams p{};
   p.mapping = a->mapping;
   p.pairs = a->num_pairs;
   p.nblocks = a->num_blocks;
-  p.bytes = a->block_bytes;
-  for (int64_t i = 0; i < a->num_arrays; i += kCopyArrays) {
-    const int64_t left = a->num_arrays - i;
-    p.arrays = (int)(left < kCopyArrays ? left : kCopyArrays);
-    for (int k = 0; k < p.arrays; ++k) p.base[k] = a->arrays[i + k];
+  p.bytes = a->num_caches > 0 ? a->block_bytes : 16;  // scales alone: one piece each
+  p.row_bytes = a->row_bytes;
+  for (int64_t i = 0; i < arrays; i += kCopyArrays) {
+    p.arrays = (int)(arrays - i < kCopyArrays ? arrays - i : kCopyArrays);
+    p.caches = (int)(a->num_caches - i < 0 ? 0 : (a->num_caches - i < p.arrays ? a->num_caches - i : p.arrays));
+    for (int k = 0; k < p.arrays; ++k) p.base[k] = array(i + k);
     const int r = copy_launch(p, static_cast<hipStream_t>(stream));
     if (r != CA_OK) return r;
   }

@@ -678,46 +678,68 @@ static PyObject* b_store_fp8(PyObject*, PyObject* const* args, Py_ssize_t nargs)
   END_HANDLE_TH_ERRORS
 }
 
-// copy_blocks(rt, arrays, mapping): pages mapping[i][0] -> mapping[i][1] (int64 [pairs, 2])
-// within each tensor of the list `arrays` (contiguous, the same shape and type, pages along
-// dim 0).  True, or None.
+// copy_blocks(rt, key_caches, value_caches, key_scales, value_scales, mapping): pages
+// mapping[i][0] -> mapping[i][1] (int64 [pairs, 2]) within each cache of the two lists
+// (contiguous [blocks, heads, page, dim] of one shape and type) and, for 8-bit caches,
+// each scale tensor ([blocks, heads]; None otherwise).  True, or None.
 static PyObject* b_copy_blocks(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
   HANDLE_TH_ERRORS
-  if (nargs != 3) {
-    PyErr_SetString(PyExc_TypeError, "copy_blocks takes 3 positional arguments");
+  if (nargs != 6) {
+    PyErr_SetString(PyExc_TypeError, "copy_blocks takes 6 positional arguments");
     return nullptr;
   }
   if (!ready()) return nullptr;
-  if (!PyList_Check(args[1]) || !plain(args[2])) Py_RETURN_NONE;
+  if (!PyList_Check(args[1]) || !PyList_Check(args[2]) || !plain(args[5])) Py_RETURN_NONE;
   const Py_ssize_t n = PyList_GET_SIZE(args[1]);
-  const at::Tensor& map = T(args[2]);
-  if (map.dim() != 2 || map.size(1) != 2 || map.scalar_type() != at::kLong || !map.is_contiguous()) Py_RETURN_NONE;
+  const at::Tensor& map = T(args[5]);
+  if (PyList_GET_SIZE(args[2]) != n || map.dim() != 2 || map.size(1) != 2 || map.scalar_type() != at::kLong ||
+      !map.is_contiguous())
+    Py_RETURN_NONE;
+  const bool scaled = args[3] != Py_None;
+  if (scaled != (args[4] != Py_None)) Py_RETURN_NONE;
+  if (scaled && (!PyList_Check(args[3]) || !PyList_Check(args[4]) || PyList_GET_SIZE(args[3]) != n ||
+                 PyList_GET_SIZE(args[4]) != n))
+    Py_RETURN_NONE;
   if (n == 0) Py_RETURN_TRUE;
-  std::vector<void*> ptrs(n);
+  if (!plain(PyList_GET_ITEM(args[1], 0))) Py_RETURN_NONE;
+  const at::Tensor& first = T(PyList_GET_ITEM(args[1], 0));
+  const at::ScalarType dt = first.scalar_type();
+  if (!(is_dtype(dt) || dt == at::kFloat8_e4m3fn) || (dt == at::kFloat8_e4m3fn) != scaled || first.dim() != 4 ||
+      !is_hd(first.size(3)) || !first.is_cuda())
+    Py_RETURN_NONE;
+  std::vector<void*> caches(2 * n), scales(scaled ? 2 * n : 0);
   for (Py_ssize_t i = 0; i < n; ++i) {
-    PyObject* o = PyList_GET_ITEM(args[1], i);
-    if (!plain(o)) Py_RETURN_NONE;
-    const at::Tensor& t = T(o);
-    const at::Tensor& first = T(PyList_GET_ITEM(args[1], 0));
-    if (t.dim() < 1 || !t.is_contiguous() || t.sizes() != first.sizes() || t.scalar_type() != first.scalar_type() ||
-        !t.is_cuda() || t.device() != first.device())
-      Py_RETURN_NONE;
-    ptrs[i] = t.data_ptr();
+    PyObject *ko = PyList_GET_ITEM(args[1], i), *vo = PyList_GET_ITEM(args[2], i);
+    if (!caches_ok(ko, vo, dt, first.size(1), first.size(3))) Py_RETURN_NONE;
+    const at::Tensor& k = T(ko);
+    const at::Tensor& v = T(vo);
+    if (k.sizes() != first.sizes() || k.device() != first.device() || v.device() != first.device()) Py_RETURN_NONE;
+    caches[2 * i] = k.data_ptr();
+    caches[2 * i + 1] = v.data_ptr();
+    if (scaled) {
+      PyObject *kso = PyList_GET_ITEM(args[3], i), *vso = PyList_GET_ITEM(args[4], i);
+      if (!scales_ok(kso, vso, k)) Py_RETURN_NONE;
+      scales[2 * i] = T(kso).data_ptr();
+      scales[2 * i + 1] = T(vso).data_ptr();
+    }
   }
-  const at::Tensor& t = T(PyList_GET_ITEM(args[1], 0));
-  if (map.size(0) == 0 || t.numel() == 0) Py_RETURN_TRUE;
-  const at::Device dev = t.device();
+  if (map.device() != first.device() && !map.device().is_cpu()) Py_RETURN_NONE;
+  if (map.size(0) == 0 || first.numel() == 0) Py_RETURN_TRUE;
+  const at::Device dev = first.device();
   const c10::DeviceGuard guard(dev);
   void* stream;
   if (!stream_of(dev, &stream)) return nullptr;
   const at::Tensor mapping = index_on(map, dev);
   ca_copy_blocks_args a{};
-  a.arrays = ptrs.data();
-  a.num_arrays = n;
-  a.block_bytes = (int64_t)t.nbytes() / t.size(0);
+  a.caches = caches.data();
+  a.num_caches = 2 * n;
+  a.block_bytes = (int64_t)first.nbytes() / first.size(0);
+  a.scales = scaled ? scales.data() : nullptr;
+  a.num_scales = scaled ? 2 * n : 0;
+  a.row_bytes = 4 * first.size(1);
   a.mapping = mapping.data_ptr<int64_t>();
   a.num_pairs = map.size(0);
-  a.num_blocks = t.size(0);
+  a.num_blocks = first.size(0);
   const int rc = g_lib.copy_blocks(&a, stream);
   if (rc == CA_DECLINED) Py_RETURN_NONE;
   if (rc != CA_OK) return failed(rc, "copy_blocks");

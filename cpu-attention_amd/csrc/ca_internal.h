@@ -87,8 +87,9 @@ constexpr int kCopyArrays = 128;  // arrays of one launch
 struct CopyParams {
   const int64_t* mapping;  // [pairs, 2]: source and destination page
   int64_t pairs, nblocks;
-  int64_t bytes;           // of a page in each array
-  int arrays;
+  int64_t bytes;           // of a page in each of the first `caches` arrays
+  int64_t row_bytes;       // of a page's scales in each of the others
+  int caches, arrays;
   void* base[kCopyArrays];
 };
 

@@ -298,17 +298,21 @@ typedef struct ca_store_fp8_args {
 int64_t ca_store_fp8_workspace_bytes(int64_t num_tokens, int64_t num_blocks, int64_t page_size);
 int ca_store_fp8(const ca_store_fp8_args* args, void* stream);
 
-/* Pages copied within each of `num_arrays` arrays of num_blocks pages of block_bytes
- * bytes (a multiple of 4; 16-byte aligned if a multiple of 16): for pair i of mapping (device, [num_pairs, 2]),
- * page mapping[2i] to page mapping[2i + 1].  `arrays` is a host array of device
- * pointers, read before the call returns.  A pair with a negative page, or of a page with itself,
- * copies nothing, and so does one past num_blocks.  Destinations must be distinct and
- * no page both a source and a destination of two pairs: such pages end up with
- * unspecified bytes. */
+/* Pages copied within each of `num_caches` arrays of num_blocks pages of block_bytes bytes
+ * (16-byte aligned, a multiple of 16) and, with them, rows of row_bytes bytes (a
+ * multiple of 4) within each of `num_scales` arrays of num_blocks rows: for pair i of
+ * mapping (device, [num_pairs, 2]), page mapping[2i] to page mapping[2i + 1].  `caches`
+ * and `scales` are host arrays of device pointers, read before the call returns.  A pair
+ * with a negative page, or of a page with itself, copies nothing, and so does one past
+ * num_blocks.  Destinations must be distinct and no page both a source and a destination
+ * of two pairs: such pages end up with unspecified bytes. */
 typedef struct ca_copy_blocks_args {
-  void* const* arrays;
-  int64_t num_arrays;
+  void* const* caches;
+  int64_t num_caches;
   int64_t block_bytes;
+  void* const* scales; /* NULL: none */
+  int64_t num_scales;
+  int64_t row_bytes;
   const int64_t* mapping;
   int64_t num_pairs;
   int64_t num_blocks;

@@ -118,11 +118,13 @@ def test_captured(cuda):
 
 def test_bindings_agree(cuda):
     mapping = torch.tensor([[0, 3], [1, 4]], device=cuda)
-    a, b = caches(2, 8, 2, 16, 64, F8)[0], caches(2, 8, 2, 16, 64, F8)[0]
-    assert K.module().copy_blocks(K.runtime(), a, mapping) is True
-    assert K.ctypes_module().copy_blocks(K.runtime(), b, mapping) is True
-    assert all(same_bytes(x, y) for x, y in zip(a, b))
+    a, b = caches(2, 8, 2, 16, 64, F8), caches(2, 8, 2, 16, 64, F8)
+    assert K.module().copy_blocks(K.runtime(), *a, mapping) is True
+    assert K.ctypes_module().copy_blocks(K.runtime(), *b, mapping) is True
+    assert all(same_bytes(x, y) for xs, ys in zip(a, b) for x, y in zip(xs, ys))
     for mod in (K.module(), K.ctypes_module()):
-        assert mod.copy_blocks(K.runtime(), a, mapping.int()) is None
-        assert mod.copy_blocks(K.runtime(), [a[0], a[1].view(torch.uint8)], mapping) is None
-        assert mod.copy_blocks(K.runtime(), [], mapping) is True
+        assert mod.copy_blocks(K.runtime(), *a, mapping.int()) is None
+        assert mod.copy_blocks(K.runtime(), a[0], a[1], None, None, mapping) is None  # 8-bit, no scales
+        assert mod.copy_blocks(K.runtime(), a[0], a[1][:1], a[2], a[3], mapping) is None
+        assert mod.copy_blocks(K.runtime(), a[0], a[1], a[2], a[2], mapping) is None  # K's scales for V
+        assert mod.copy_blocks(K.runtime(), [], [], None, None, mapping) is True

@@ -256,7 +256,7 @@ def test_module_entries_decline_with_none(binding):
         assert mod.decode_window(rt, q, kc, vc, *s, None, None, lens, table, None, 3, 1, 0) is None
     x = torch.randn(3, 4, 64)
     assert mod.store_fp8(rt, x, x, kc, vc, *scales, torch.arange(3)) is None
-    assert mod.copy_blocks(rt, [kc, vc], torch.tensor([[0, 1]])) is None
+    assert mod.copy_blocks(rt, [kc], [vc], *[[x] for x in scales], torch.tensor([[0, 1]])) is None
     if isinstance(mod, K.NativeModule):
         for entry in (mod.flash_window, mod.decode_window, mod.store_fp8, mod.copy_blocks):
             with pytest.raises(TypeError):
@@ -332,11 +332,13 @@ def test_library_declines_malformed_calls_without_a_gpu():
     assert rc("ca_store_fp8", s) == K.CA_OK
     t.page_size = 24
     assert rc("ca_store_fp8", s) == K.CA_DECLINED
-    c = K.CopyBlocksArgs(num_arrays=1, block_bytes=64, num_pairs=1, num_blocks=2)
+    c = K.CopyBlocksArgs(num_caches=1, block_bytes=64, num_pairs=1, num_blocks=2)
     assert rc("ca_copy_blocks", c) == K.CA_DECLINED  # null pointers
     c.num_pairs = 0
     assert rc("ca_copy_blocks", c) == K.CA_OK
-    c.block_bytes = 6
+    c.block_bytes = 24
+    assert rc("ca_copy_blocks", c) == K.CA_DECLINED
+    c.block_bytes, c.num_scales, c.row_bytes = 64, 1, 6
     assert rc("ca_copy_blocks", c) == K.CA_DECLINED
 
 
