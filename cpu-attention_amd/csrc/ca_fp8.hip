@@ -42,7 +42,10 @@ constexpr int kStore8Waves = 4;       // heads per block
 // Blocks that walk the listed pages: one unit each up to here (128 prompts of 64 to 1024
 // tokens, H=32 E=128, 35000 units: 4096 blocks 442 us, 16384 425, 65536 420, more the same).
 constexpr int64_t kStore8Grid = 65536;
-constexpr int64_t kScanTokens = 1024;  // tokens up to which each block scans the slots
+// Tokens up to which each block scans the slots (scan / list, E=128 page 16: 256 tokens H=8
+// 6.5 / 10.4 us, H=32 10.0 / 11.2; 512 8.9 / 10.7 and 13.6 / 12.3; 1024 16.3 / 11.0 and 25.3 /
+// 13.7).
+constexpr int64_t kScanTokens = 512;
 constexpr int64_t kScanPage = 1024;    // positions of a page up to which it can
 
 // The smallest power of two from 2^-100 that takes magnitudes up to `top` (finite) to 448
@@ -250,10 +253,10 @@ __global__ __launch_bounds__(64 * kStore8Waves) void store8_scan_kernel(Store8Pa
   __syncthreads();
   bool earlier = false;
   for (int64_t j = threadIdx.x; j < p.ntok; j += 64 * kStore8Waves) {
-    const int64_t s = p.slots[j];
-    if (slot_page(p, s) == blk) {
+    const int64_t t = p.slots[j] - blk * p.page;
+    if (t >= 0 && t < p.page) {
       earlier |= j < i;
-      atomicMax(&owner[s - blk * p.page], (int)j);
+      atomicMax(&owner[t], (int)j);
     }
   }
   if (__syncthreads_or(earlier) || h >= p.heads) return;
