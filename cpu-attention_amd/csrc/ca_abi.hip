@@ -400,7 +400,8 @@ extern "C" int64_t ca_decode_window_workspace_bytes(int64_t num_seqs, int64_t nu
   if (num_seqs < 0 || num_heads < 0 || page_size <= 0 || page_table_width < 0 || sinks < 0) return -1;
   const int64_t cap = page_table_width * page_size;
   const int64_t tiles = win_decode_tiles(page_table_width, page_size, win_left(left, cap), sinks < cap ? sinks : cap);
-  return win_decode_ws_bytes(win_decode_slots(num_seqs * num_heads, tiles), head_dim);
+  // One tile more: an 8-bit cache's last page, if the call appends to it.
+  return win_decode_ws_bytes(win_decode_slots(num_seqs * num_heads, tiles + 1), head_dim);
 }
 
 extern "C" int ca_decode_window(const ca_decode_window_args* wa, void* stream) {
@@ -426,7 +427,8 @@ extern "C" int ca_decode_window(const ca_decode_window_args* wa, void* stream) {
   WinDecodeParams p{};
   p.left = win_left(wa->left, cap);
   p.sinks = wa->sinks < cap ? wa->sinks : cap;
-  const int64_t tiles = win_decode_tiles(a->page_table_width, a->page_size, p.left, p.sinks);
+  const bool fold = a->k_new && per_seq == 1 && win_decode_folds(rows, a->page_size, f8);
+  const int64_t tiles = win_decode_tiles(a->page_table_width, a->page_size, p.left, p.sinks) + (fold && f8 ? 1 : 0);
   if (tiles > 0x7fffffff) return CA_DECLINED;
   p.tiles = (int)tiles;
   p.slots = win_decode_slots(rows, p.tiles);
@@ -434,8 +436,17 @@ extern "C" int ca_decode_window(const ca_decode_window_args* wa, void* stream) {
                       a->workspace_bytes < win_decode_ws_bytes(p.slots, a->head_dim)))
     return CA_DECLINED;
   hipStream_t st = static_cast<hipStream_t>(stream);
-  // The new tokens go in first, by a kernel of their own.
-  if (a->k_new) {
+  // One new token per sequence is stored by the decode itself in small calls, others go in
+  // first, by a kernel of their own.
+  if (fold) {
+    p.k_new = static_cast<const uint32_t*>(a->k_new);
+    p.v_new = static_cast<const uint32_t*>(a->v_new);
+    p.new_stride = a->kv_stride;
+    p.kc_store = static_cast<uint32_t*>(a->k_cache);
+    p.vc_store = static_cast<uint32_t*>(a->v_cache);
+    p.k_scale_store = wa->k_scale;
+    p.v_scale_store = wa->v_scale;
+  } else if (a->k_new) {
     int r;
     if (f8) {
       Store8Params sp{};

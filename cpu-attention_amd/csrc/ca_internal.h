@@ -63,10 +63,14 @@ struct WinDecodeParams : DecodeParams {
   int64_t sinks;          // first keys that stay visible
   const float* k_scale;   // [nblocks, heads], nullptr: the cache holds q's type
   const float* v_scale;
+  // The one-token append done inside the decode (k_new of DecodeParams; nullptr: none).
+  int64_t new_stride;     // elements from one sequence's new token to the next's
+  float* k_scale_store;   // the scales, writable
+  float* v_scale_store;
 };
 
-// Tokens into the cache of e4m3 codes (ca_fp8.hip).
-struct Store8Params {
+// A cache of e4m3 codes and the tokens that go into it.
+struct Store8Page {
   const void* key;        // [T, H, E] rows, token stride tok_stride (elements)
   const void* value;
   int64_t tok_stride;
@@ -74,11 +78,16 @@ struct Store8Params {
   uint32_t* vc;           // per (block, head): P rows of E/4 words
   float* k_scale;         // [nblocks, heads]
   float* v_scale;
+  int64_t heads, page;
+};
+
+// Tokens into the cache of e4m3 codes (ca_fp8.hip).
+struct Store8Params : Store8Page {
   const int64_t* slots;   // slot mode: [T]; nullptr selects append mode
   const int32_t* lens;    // append mode: [T / per_seq] positions
   const int32_t* page_table;
   int64_t pt_width;
-  int64_t ntok, heads, page, nblocks, per_seq;
+  int64_t ntok, nblocks, per_seq;
   int32_t* work;          // slot mode of many tokens: store8_work_ints() of them
 };
 
@@ -297,6 +306,8 @@ int64_t win_decode_slots(int64_t rows, int64_t tiles);
 int win_decode_launch(const WinDecodeParams& p, int head_dim, int bf16, hipStream_t stream);
 // 32-bit words of scratch that a store of these sizes needs (0: none).
 int64_t store8_work_ints(int64_t ntok, int64_t nblocks, int64_t page);
+// Whether a decode of these sizes stores its one new token per sequence itself.
+bool win_decode_folds(int64_t rows, int64_t page, bool fp8);
 int store8_launch(const Store8Params& p, int head_dim, int bf16, hipStream_t stream);
 int copy_launch(const CopyParams& p, hipStream_t stream);
 // ca_decode_noalloc's scratch on the current device (and that device's index),

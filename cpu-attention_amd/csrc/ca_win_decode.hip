@@ -17,6 +17,7 @@
 //
 // Bound: reading the visible keys once (HBM).
 #include "ca_device.h"
+#include "ca_fp8.h"
 #include "ca_internal.h"
 #include "ca_merge.h"
 
@@ -27,9 +28,15 @@ constexpr int kWinTile = 64;  // keys per tile
 
 // The units that row `seq` walks: units 0 .. su - 1 hold the sinks, unit i >= su of the
 // walk is unit i - su + u0 of the sequence; nu in all.
+//
+// The walk's tiles take TK / 16 units each, the last one the units from `last` on.  A call
+// that appends to an 8-bit cache in this kernel (FOLD) gives the last page's units, at
+// most 4, a tile of their own: the wave that takes it may rescale the page, and nobody else
+// may read it then.
 struct Span {
-  int64_t len, lo, s, su, u0, nu;
+  int64_t len, lo, s, su, u0, nu, last, tiles;
 };
+template <bool FOLD>
 __device__ __forceinline__ Span span_of(const WinDecodeParams& p, int64_t seq) {
   const int64_t cap = p.pt_width * p.page;
   Span x;
@@ -40,6 +47,15 @@ __device__ __forceinline__ Span span_of(const WinDecodeParams& p, int64_t seq) {
   x.su = cdiv(x.s, kUnit);
   x.u0 = max<int64_t>(x.lo / kUnit, x.su);
   x.nu = x.su + max<int64_t>(0, cdiv(x.len, kUnit) - x.u0);
+  constexpr int NU = kWinTile / kUnit;
+  if (FOLD) {
+    const int64_t lp = x.len > 0 ? (x.len - 1) / p.page * (p.page / kUnit) : 0;  // the last page's first unit
+    x.last = lp < x.su ? lp : x.su + max<int64_t>(0, lp - x.u0);
+    x.tiles = cdiv(x.last, NU) + 1;
+  } else {
+    x.last = x.nu > 0 ? (x.nu - 1) / NU * NU : 0;
+    x.tiles = x.last / NU + 1;
+  }
   return x;
 }
 
@@ -57,11 +73,11 @@ struct WinShape {
   static constexpr int G = kWave / LPR;              // V rows per wave load
 };
 
-// Tile `tile` (units tile * TK / 16 ...) of row (seq, h): leaves the wave's partial
-// state (P.V, max in scaled log2 units, sum) in part[E + 2].
-template <int E, bool BF, bool F8, int TK>
+// Tile `tile` of row (seq, h): leaves the wave's partial state (P.V, max in scaled log2
+// units, sum) in part[E + 2].  APPEND: the row's last tile stores the call's new token.
+template <int E, bool BF, bool F8, bool APPEND, int TK>
 __device__ __forceinline__ void win_tile(const WinDecodeParams& p, const Span& sp, int64_t seq, int64_t h, int64_t tile,
-                                         float* p_lds, float* part) {
+                                         float* p_lds, float* part, uint32_t* kl) {
   using D = WinShape<E, BF, F8>;
   constexpr int W = D::W, DPL = D::DPL, LPR = D::LPR, G = D::G, CES = D::CES;
   constexpr int NU = TK / kUnit, NQ = TK / 4, SPLIT = kWave / NQ, WPL = W / SPLIT;
@@ -73,8 +89,34 @@ __device__ __forceinline__ void win_tile(const WinDecodeParams& p, const Span& s
   int64_t kb = 0, vb = 0;
   uint32_t vis = 0;
   float ksc = 1.f, vsc = 1.f;
-  const int64_t iu = tile * NU + lane;
-  if (lane < NU && iu < sp.nu) {
+  const bool final = tile == sp.tiles - 1;
+  const int64_t iu = (final ? sp.last : tile * NU) + lane;
+  // The new token: at position lens[seq], the row's newest unless that lies past the table.
+  const bool fresh = APPEND && final && sp.len > 0 && p.lens[seq] == sp.len - 1;
+  if constexpr (APPEND && F8) {
+    if (fresh) {
+      const int64_t pi = (sp.len - 1) / p.page, at = sp.len - 1 - pi * p.page;
+      const int64_t blk = p.page_table[seq * p.pt_width + pi];
+      if (blk >= 0 && blk < p.nblocks) {
+        Store8Page s;
+        s.key = p.k_new;
+        s.value = p.v_new;
+        s.tok_stride = p.new_stride;
+        s.kc = p.kc_store;
+        s.vc = p.vc_store;
+        s.k_scale = p.k_scale_store;
+        s.v_scale = p.v_scale_store;
+        s.heads = p.heads;
+        s.page = p.page;
+        store_page<E, BF>(s, blk, h, kl, [&](int64_t t) -> int { return t == at ? (int)seq : -1; });
+        // The codes and scales are read back below, by other lanes.
+        __builtin_amdgcn_fence(__ATOMIC_RELEASE, "workgroup");
+        __builtin_amdgcn_wave_barrier();
+        __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "workgroup");
+      }
+    }
+  }
+  if (lane < NU && iu < sp.nu && (final || lane < sp.last - tile * NU)) {
     const int64_t tu = (iu < sp.su ? iu : iu - sp.su + sp.u0) * kUnit;
     const int64_t pi = tu / p.page, off = tu - pi * p.page;
     const int64_t blk = p.page_table[seq * p.pt_width + pi];
@@ -92,6 +134,36 @@ __device__ __forceinline__ void win_tile(const WinDecodeParams& p, const Span& s
   uint64_t mask = 0;
 #pragma unroll
   for (int u = 0; u < NU; ++u) mask |= (uint64_t)(uint32_t)__builtin_amdgcn_readlane((int)vis, u) << (kUnit * u);
+
+  // The new token of a 16- or 32-bit cache: its words and q's, and its key in the tile.  Its
+  // logit comes from these registers and its V row from where it lies, so nothing waits
+  // for the stores to the cache.
+  constexpr int KNW = (W + kWave - 1) / kWave;
+  uint32_t knw[KNW], qnw[KNW];
+  const char* vnew = nullptr;
+  int newj = -1;
+  if constexpr (APPEND && !F8) {
+    const int last = (int)(sp.nu - 1 - sp.last);  // the tile's last unit holds it
+    if (fresh && __builtin_amdgcn_readlane((int)vis, last & (NU - 1)) != 0) {
+      newj = kUnit * last + (int)((sp.len - 1) & (kUnit - 1));
+      const int64_t src = seq * p.new_stride + h * E;
+      const uint32_t* kn = reinterpret_cast<const uint32_t*>(reinterpret_cast<const char*>(p.k_new) + src * CES);
+      const uint32_t* qw = reinterpret_cast<const uint32_t*>(reinterpret_cast<const char*>(p.q) + (seq * p.q_stride + h * E) * CES);
+      vnew = reinterpret_cast<const char*>(p.v_new) + src * CES;
+      const int64_t kbn = __shfl(kb, last), vbn = __shfl(vb, last);
+      const int x = newj & (kUnit - 1);
+#pragma unroll
+      for (int i = 0; i < KNW; ++i) {
+        const int w = lane + kWave * i;
+        knw[i] = w < W ? kn[w] : 0u;
+        qnw[i] = w < W ? qw[w] : 0u;
+        if (w < W) p.kc_store[kbn + (int64_t)w * p.page + x] = knw[i];
+      }
+      if (lane < W / 4)
+        *reinterpret_cast<u32x4*>(p.vc_store + (vbn + (int64_t)x * E) * CES / 4 + 4 * lane) =
+            *reinterpret_cast<const u32x4*>(vnew + 16 * lane);
+    }
+  }
 
   // ---- Q.K
   float s[4] = {0.f, 0.f, 0.f, 0.f};
@@ -152,6 +224,19 @@ __device__ __forceinline__ void win_tile(const WinDecodeParams& p, const Span& s
       }
     }
   }
+  float lnew = 0.f;
+  if constexpr (APPEND && !F8) {
+    if (newj >= 0) {
+#pragma unroll
+      for (int i = 0; i < KNW; ++i) {
+        if constexpr (BF)
+          lnew = __builtin_amdgcn_fdot2_f32_bf16(as_bf16x2(knw[i]), as_bf16x2(qnw[i]), lnew, false);
+        else
+          lnew = fmaf(__uint_as_float(knw[i]), __uint_as_float(qnw[i]), lnew);
+      }
+      lnew = wave_sum(lnew);
+    }
+  }
   // The SPLIT lanes of a quad sum their parts.  Scaled logits: -inf for a masked key,
   // +inf for a NaN (its row comes out NaN then; as a NaN, the maxima would skip it and
   // a tile of nothing else would count as empty).
@@ -160,6 +245,7 @@ __device__ __forceinline__ void win_tile(const WinDecodeParams& p, const Span& s
   for (int j = 0; j < 4; ++j) {
 #pragma unroll
     for (int o = NQ; o < kWave; o <<= 1) s[j] += __shfl_xor(s[j], o);
+    if (APPEND && !F8 && 4 * quad + j == newj) s[j] = lnew;
     x[j] = s[j] * cs;
     x[j] = x[j] != x[j] ? INFINITY : x[j];
     x[j] = qvis >> j & 1 ? x[j] : -INFINITY;
@@ -198,9 +284,9 @@ __device__ __forceinline__ void win_tile(const WinDecodeParams& p, const Span& s
       const int key = g + G * (b0 + i);
       ok[i] = mask >> key & 1;
       const int64_t vu = __shfl(vb, key / kUnit);
-      if (ok[i])
-        v4[i] = __builtin_nontemporal_load(
-            reinterpret_cast<const u32x4*>(vbase + (vu + (int64_t)(key & (kUnit - 1)) * E) * CES));
+      const char* at = vbase + (vu + (int64_t)(key & (kUnit - 1)) * E) * CES;
+      if (APPEND && !F8 && key == newj) at = vnew + dl * 16;
+      if (ok[i]) v4[i] = __builtin_nontemporal_load(reinterpret_cast<const u32x4*>(at));
     }
 #pragma unroll
     for (int i = 0; i < B; ++i) {
@@ -239,31 +325,31 @@ __device__ __forceinline__ void win_tile(const WinDecodeParams& p, const Span& s
   }
 }
 
-template <int E, bool BF, bool F8, int TK>
+template <int E, bool BF, bool F8, bool APPEND, int TK>
 __global__ __launch_bounds__(64 * kDecWaves) void win_decode_kernel(WinDecodeParams p) {
   __shared__ __attribute__((aligned(16))) float p_lds[kDecWaves][TK];
   __shared__ float part[kDecWaves][E + 2];
-  constexpr int NU = TK / kUnit;
+  // K's transposition of an 8-bit append: by the one wave of the row's last tile.
+  __shared__ __attribute__((aligned(16))) uint32_t kl[APPEND && F8 ? Store8Shape<E>::LDS_WORDS : 1];
   const int wv = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int64_t row = blockIdx.x;
   const int64_t s = row / p.heads, h = row - s * p.heads;
   const int64_t tile = (int64_t)blockIdx.y * kDecWaves + wv;
-  const Span sp = span_of(p, s);
-  // Waves past the row's last unit exit (the barrier below waits for the others only);
-  // the row's first wave stays, and writes a row with no key as exactly 0.
-  if (tile * NU >= sp.nu && tile != 0) return;
-  win_tile<E, BF, F8, TK>(p, sp, s, h, tile, p_lds[wv], part[wv]);
+  const Span sp = span_of<APPEND && F8>(p, s);
+  // Waves past the row's last tile exit (the barrier below waits for the others only).  A
+  // row with no key has one tile of nothing, and is written as exactly 0.
+  if (tile >= sp.tiles) return;
+  win_tile<E, BF, F8, APPEND, TK>(p, sp, s, h, tile, p_lds[wv], part[wv], kl);
   __syncthreads();
   if (wv != 0) return;
   constexpr int DPC = E >= 64 ? E / 64 : 1;
   const int lane = threadIdx.x & 63;
-  const int64_t tiles = max<int64_t>(1, cdiv(sp.nu, NU));
-  const int n = (int)min<int64_t>(kDecWaves, tiles - (int64_t)blockIdx.y * kDecWaves);
+  const int n = (int)min<int64_t>(kDecWaves, sp.tiles - (int64_t)blockIdx.y * kDecWaves);
   float mx, acc[DPC];
   const float l = merge_states<E, DPC>(n, [&](int t, int i) {
     return part[t][i == -1 ? E : (i == -2 ? E + 1 : i)];
   }, mx, acc);
-  if (tiles <= kDecWaves) {
+  if (sp.tiles <= kDecWaves) {
     if (lane * DPC < E) store_out<DPC, BF>(p.out, row * E + lane * DPC, acc, l > 0.f ? 1.f / l : 0.f);
     return;
   }
@@ -279,18 +365,19 @@ __global__ __launch_bounds__(64 * kDecWaves) void win_decode_kernel(WinDecodePar
 }
 
 // One wave per row of more than one block: merges the blocks' partials.
-template <int E, bool BF, int TK>
+template <int E, bool BF, bool FOLD>
 __global__ __launch_bounds__(256) void win_decode_combine_kernel(WinDecodeParams p) {
   const int lane = threadIdx.x & 63;
   const int64_t row = (int64_t)blockIdx.x * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   if (row >= p.nseqs * p.heads) return;
-  const int64_t tiles = cdiv(span_of(p, row / p.heads).nu, TK / kUnit);
+  const int64_t tiles = span_of<FOLD>(p, row / p.heads).tiles;
   if (tiles <= kDecWaves) return;  // written by its block
   merge_partials<E, BF, false>(p, row, (int)cdiv(tiles, kDecWaves), lane);
 }
 
 // The most tiles that a row can have: its page table's capacity, or the units of the
-// sinks and of a window that begins at any key of its first unit.
+// sinks and of a window that begins at any key of its first unit.  (FOLD: one more, for the
+// last page's own tile.)
 int64_t win_decode_tiles(int64_t pt_width, int64_t page, int64_t left, int64_t sinks) {
   int64_t units = pt_width * page / kUnit;
   if (left >= 0) {
@@ -298,6 +385,12 @@ int64_t win_decode_tiles(int64_t pt_width, int64_t page, int64_t left, int64_t s
     units = units < seen ? units : seen;
   }
   return cdiv(units, kWinTile / kUnit);
+}
+
+// The decode stores a new token itself for up to kFusedAppendMaxRows rows (as ca_decode), if
+// the page of an 8-bit cache fits a tile.
+bool win_decode_folds(int64_t rows, int64_t page, bool fp8) {
+  return rows <= kFusedAppendMaxRows && (!fp8 || page <= kWinTile);
 }
 
 // Partial slots: one per (row, block of 8 tiles) when rows can outgrow one block.
@@ -308,11 +401,18 @@ static int win_decode_launch_t(const WinDecodeParams& p, hipStream_t stream) {
   const int64_t rows = p.nseqs * p.heads;
   const int64_t gy = p.tiles > kDecWaves ? cdiv(p.tiles, kDecWaves) : 1;
   if (rows > 0x7fffffff || gy > 65535 || win_decode_slots(rows, p.tiles) > p.slots) return CA_DECLINED;
-  hipLaunchKernelGGL((win_decode_kernel<E, BF, F8, kWinTile>), dim3((unsigned)rows, (unsigned)gy), dim3(64 * kDecWaves),
-                     0, stream, p);
+  const dim3 grid((unsigned)rows, (unsigned)gy), block(64 * kDecWaves);
+  if (p.k_new)
+    hipLaunchKernelGGL((win_decode_kernel<E, BF, F8, true, kWinTile>), grid, block, 0, stream, p);
+  else
+    hipLaunchKernelGGL((win_decode_kernel<E, BF, F8, false, kWinTile>), grid, block, 0, stream, p);
   const int st = ca_launch_status();
   if (st != CA_OK || gy == 1) return st;
-  hipLaunchKernelGGL((win_decode_combine_kernel<E, BF, kWinTile>), dim3((unsigned)cdiv(rows, 4)), dim3(256), 0, stream, p);
+  const dim3 cg((unsigned)cdiv(rows, 4));
+  if (F8 && p.k_new)
+    hipLaunchKernelGGL((win_decode_combine_kernel<E, BF, true>), cg, dim3(256), 0, stream, p);
+  else
+    hipLaunchKernelGGL((win_decode_combine_kernel<E, BF, false>), cg, dim3(256), 0, stream, p);
   return ca_launch_status();
 }
 
