@@ -25,6 +25,15 @@ namespace ca {
 
 constexpr int kUnit = 16;     // keys per unit: never straddles a page
 constexpr int kWinTile = 64;  // keys per tile
+// V rows of a lane up to which they are loaded before the logits.  4 (8-bit E = 32 and 64,
+// bf16 E = 32) hide a load's latency for few registers (8-bit fp32 N=8 H=16 E=64 14.1 -> 13.1
+// us); 8 take 8-bit E = 128 to 129 registers and one block per CU (N=64 H=32, lengths to
+// 4095: 193 -> 284 us), 16 bf16 E = 64 the same way (52 -> 61 us).
+constexpr int kEarlyRows = 4;
+
+// Positions and pages fit 32 unsigned bits (lengths are 32-bit, plus at most 2^30 new
+// tokens; the launcher bounds the page), and a 32-bit division takes a third of a 64-bit one.
+__device__ __forceinline__ int64_t page_of(int64_t pos, int64_t page) { return (uint32_t)pos / (uint32_t)page; }
 
 // The units that row `seq` walks: units 0 .. su - 1 hold the sinks, unit i >= su of the
 // walk is unit i - su + u0 of the sequence; nu in all.
@@ -49,7 +58,7 @@ __device__ __forceinline__ Span span_of(const WinDecodeParams& p, int64_t seq) {
   x.nu = x.su + max<int64_t>(0, cdiv(x.len, kUnit) - x.u0);
   constexpr int NU = kWinTile / kUnit;
   if (FOLD) {
-    const int64_t lp = x.len > 0 ? (x.len - 1) / p.page * (p.page / kUnit) : 0;  // the last page's first unit
+    const int64_t lp = x.len > 0 ? page_of(x.len - 1, p.page) * (p.page / kUnit) : 0;  // the last page's first unit
     x.last = lp < x.su ? lp : x.su + max<int64_t>(0, lp - x.u0);
     x.tiles = cdiv(x.last, NU) + 1;
   } else {
@@ -95,7 +104,7 @@ __device__ __forceinline__ void win_tile(const WinDecodeParams& p, const Span& s
   const bool fresh = APPEND && final && sp.len > 0 && p.lens[seq] == sp.len - 1;
   if constexpr (APPEND && F8) {
     if (fresh) {
-      const int64_t pi = (sp.len - 1) / p.page, at = sp.len - 1 - pi * p.page;
+      const int64_t pi = page_of(sp.len - 1, p.page), at = sp.len - 1 - pi * p.page;
       const int64_t blk = p.page_table[seq * p.pt_width + pi];
       if (blk >= 0 && blk < p.nblocks) {
         Store8Page s;
@@ -118,7 +127,7 @@ __device__ __forceinline__ void win_tile(const WinDecodeParams& p, const Span& s
   }
   if (lane < NU && iu < sp.nu && (final || lane < sp.last - tile * NU)) {
     const int64_t tu = (iu < sp.su ? iu : iu - sp.su + sp.u0) * kUnit;
-    const int64_t pi = tu / p.page, off = tu - pi * p.page;
+    const int64_t pi = page_of(tu, p.page), off = tu - pi * p.page;
     const int64_t blk = p.page_table[seq * p.pt_width + pi];
     if (blk >= 0 && blk < p.nblocks) {
       vis = low_bits(sp.len - tu) & (low_bits(sp.s - tu) | ~low_bits(sp.lo - tu));
@@ -165,20 +174,42 @@ __device__ __forceinline__ void win_tile(const WinDecodeParams& p, const Span& s
     }
   }
 
+  // V rows: lane group g reads rows g, g + G, ... of the tile, lane dl of it 16 bytes.  Where
+  // a lane's rows fit the registers (EARLY) they are loaded before the logits, beside K.
+  constexpr int R = TK / G, B = R < 16 ? R : 16;
+  constexpr bool EARLY = R <= kEarlyRows;
+  const int g = lane / LPR, dl = lane - g * LPR;
+  u32x4 v4[B];
+  auto load_v = [&](int b0) __attribute__((always_inline)) {
+#pragma unroll
+    for (int i = 0; i < B; ++i) {
+      const int key = g + G * (b0 + i);
+      const int64_t vu = __shfl(vb, key / kUnit);
+      const char* at = reinterpret_cast<const char*>(p.vc) + (vu + (int64_t)(key & (kUnit - 1)) * E) * CES;
+      if (APPEND && !F8 && key == newj) at = vnew;
+      if (mask >> key & 1) v4[i] = __builtin_nontemporal_load(reinterpret_cast<const u32x4*>(at + dl * 16));
+    }
+  };
+
   // ---- Q.K
   float s[4] = {0.f, 0.f, 0.f, 0.f};
   const uint32_t qvis = (uint32_t)(mask >> (4 * quad)) & 15u;
   const int64_t kbu = __shfl(kb, quad >> 2);
   float cs = p.c;
   if (F8) cs *= __shfl(ksc, quad >> 2);
-  if (qvis) {
-    const uint32_t* kp = p.kc + kbu + 4 * (quad & 3) + (int64_t)phase * p.page;
-    constexpr int QU = WPL < 16 ? WPL : 16;  // K loads in flight
-    for (int w0 = 0; w0 < WPL; w0 += QU) {
-      u32x4 k4[QU];
+  constexpr int QU = WPL < 16 ? WPL : 16;  // K loads in flight
+  u32x4 k4[QU];
+  const uint32_t* kp = p.kc + kbu + 4 * (quad & 3) + (int64_t)phase * p.page;
+  auto load_k = [&](int w0) __attribute__((always_inline)) {
 #pragma unroll
-      for (int i = 0; i < QU; ++i)
-        k4[i] = __builtin_nontemporal_load(reinterpret_cast<const u32x4*>(kp + (int64_t)(w0 + i) * SPLIT * p.page));
+    for (int i = 0; i < QU; ++i)
+      k4[i] = __builtin_nontemporal_load(reinterpret_cast<const u32x4*>(kp + (int64_t)(w0 + i) * SPLIT * p.page));
+  };
+  if (qvis) load_k(0);
+  if (EARLY) load_v(0);
+  if (qvis) {
+    for (int w0 = 0; w0 < WPL; w0 += QU) {
+      if (w0 > 0) load_k(w0);
 #pragma unroll
       for (int i = 0; i < QU; ++i) {
         const int w = phase + (w0 + i) * SPLIT;
@@ -268,29 +299,16 @@ __device__ __forceinline__ void win_tile(const WinDecodeParams& p, const Span& s
   if (phase == 0) *reinterpret_cast<f32x4*>(&p_lds[4 * quad]) = f32x4{pr[0], pr[1], pr[2], pr[3]};
   wave_lds_sync();
 
-  // ---- P.V: lane group g reads rows g, g + G, ... of the tile, lane dl of it 16 bytes.
-  constexpr int R = TK / G, B = R < 16 ? R : 16;
-  const int g = lane / LPR, dl = lane - g * LPR;
-  const char* vbase = reinterpret_cast<const char*>(p.vc) + dl * 16;
+  // ---- P.V
   float acc[DPL];
 #pragma unroll
   for (int i = 0; i < DPL; ++i) acc[i] = 0.f;
 #pragma unroll
   for (int b0 = 0; b0 < R; b0 += B) {
-    u32x4 v4[B];
-    bool ok[B];
+    if (!EARLY) load_v(b0);
 #pragma unroll
     for (int i = 0; i < B; ++i) {
-      const int key = g + G * (b0 + i);
-      ok[i] = mask >> key & 1;
-      const int64_t vu = __shfl(vb, key / kUnit);
-      const char* at = vbase + (vu + (int64_t)(key & (kUnit - 1)) * E) * CES;
-      if (APPEND && !F8 && key == newj) at = vnew + dl * 16;
-      if (ok[i]) v4[i] = __builtin_nontemporal_load(reinterpret_cast<const u32x4*>(at));
-    }
-#pragma unroll
-    for (int i = 0; i < B; ++i) {
-      if (ok[i]) {
+      if (mask >> (g + G * (b0 + i)) & 1) {
         const float pj = p_lds[g + G * (b0 + i)];
 #pragma unroll
         for (int x4 = 0; x4 < 4; ++x4) {
@@ -333,7 +351,7 @@ __global__ __launch_bounds__(64 * kDecWaves) void win_decode_kernel(WinDecodePar
   __shared__ __attribute__((aligned(16))) uint32_t kl[APPEND && F8 ? Store8Shape<E>::LDS_WORDS : 1];
   const int wv = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int64_t row = blockIdx.x;
-  const int64_t s = row / p.heads, h = row - s * p.heads;
+  const int64_t s = (uint32_t)row / (uint32_t)p.heads, h = row - s * p.heads;
   const int64_t tile = (int64_t)blockIdx.y * kDecWaves + wv;
   const Span sp = span_of<APPEND && F8>(p, s);
   // Waves past the row's last tile exit (the barrier below waits for the others only).  A
@@ -400,7 +418,7 @@ template <int E, bool BF, bool F8>
 static int win_decode_launch_t(const WinDecodeParams& p, hipStream_t stream) {
   const int64_t rows = p.nseqs * p.heads;
   const int64_t gy = p.tiles > kDecWaves ? cdiv(p.tiles, kDecWaves) : 1;
-  if (rows > 0x7fffffff || gy > 65535 || win_decode_slots(rows, p.tiles) > p.slots) return CA_DECLINED;
+  if (rows > 0x7fffffff || p.page > 0x7fffffff || gy > 65535 || win_decode_slots(rows, p.tiles) > p.slots) return CA_DECLINED;
   const dim3 grid((unsigned)rows, (unsigned)gy), block(64 * kDecWaves);
   if (p.k_new)
     hipLaunchKernelGGL((win_decode_kernel<E, BF, F8, true, kWinTile>), grid, block, 0, stream, p);
