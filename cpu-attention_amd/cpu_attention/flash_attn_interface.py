@@ -38,6 +38,7 @@ _REFUSED = ("cpu_attention: qv, rotary, cache_leftpad, varlen, descale, sliding 
             "windows, softcap, attention_chunk, alibi and return_softmax_lse are not supported")
 _NEW_TOKENS = "cpu_attention: k/v must both be [batch, seqlen_new, nheads, headdim]"
 _ENTRIES = []  # [runtime handle, module decode, module flash] once the library is loaded
+_WINDOW_ENTRIES = []  # [runtime handle, module flash_window, module decode_window], as well
 
 
 def _entries():
@@ -45,6 +46,13 @@ def _entries():
         mod = K.module()
         _ENTRIES.extend((K.runtime(), mod.decode, mod.flash))
     return _ENTRIES
+
+
+def _window_entries():
+    if not _WINDOW_ENTRIES:
+        mod = K.module()
+        _WINDOW_ENTRIES.extend((K.runtime(), mod.flash_window, mod.decode_window))
+    return _WINDOW_ENTRIES
 
 
 def _as_plain(x):
@@ -305,14 +313,22 @@ def _check_flash(q, k, v):
     return readable
 
 
+_FAR = 1 << 62
+
+
 def _window_options(window_size, sink_tokens, softmax_scale):
     """The window's (left, right) and the sinks as whole numbers, checked."""
+    if type(window_size) is tuple and len(window_size) == 2:  # the usual call, in a few comparisons
+        left, right = window_size
+        if type(left) is type(right) is type(sink_tokens) is int and -1 <= left < _FAR and -1 <= right < _FAR \
+                and 0 <= sink_tokens < _FAR and softmax_scale is None:
+            return left, right, sink_tokens
     try:
         left, right = (operator.index(x) for x in window_size)
         sinks = operator.index(sink_tokens)
     except (TypeError, ValueError):
         raise ValueError("cpu_attention: window_size must be two ints and sink_tokens an int") from None
-    if left < -1 or right < -1 or sinks < 0 or max(left, right, sinks) >= 1 << 62:
+    if left < -1 or right < -1 or sinks < 0 or max(left, right, sinks) >= _FAR:
         raise ValueError("cpu_attention: window_size must be -1 (no limit) or more on each side, "
                          "sink_tokens 0 or more")
     if softmax_scale is not None and not 0.0 < float(softmax_scale) < math.inf:
@@ -333,7 +349,7 @@ def flash_attn_window_func(q, k, v, window_size=(-1, -1), sink_tokens=0, softmax
     ``flash_attn_func``'s; ``softmax_scale`` must be positive and finite.
     """
     left, right, sinks = _window_options(window_size, sink_tokens, softmax_scale)
-    flash, rt = K.module().flash_window, K.runtime()
+    rt, flash, _ = _WINDOW_ENTRIES or _window_entries()
     out = flash(rt, q, k, v, softmax_scale, causal, left, right, sinks)
     if out is None:
         q, k, v = _check_flash(q, k, v)
@@ -435,7 +451,7 @@ def _decode_window(q, k_cache, v_cache, k_scale, v_scale, k, v, lens, page_table
             k, v, n = None, None, 1
         else:  # rows of [seqs * n, heads, dim]
             k, v = k.reshape(-1, *k.shape[2:]), v.reshape(-1, *v.shape[2:])
-    decode, rt = K.module().decode_window, K.runtime()
+    rt, _, decode = _WINDOW_ENTRIES or _window_entries()
     out = decode(rt, q, k_cache, v_cache, k_scale, v_scale, k, v, lens, page_table, scale, left, sinks, n)
     if out is None:
         q, k_cache, v_cache, k_scale, v_scale, k, v, page_table, lens = _check_window_kvcache(

@@ -345,7 +345,7 @@ __global__ __launch_bounds__(256 * KG, (DuoCfg<E, KG>::WAVES)) void flash_duo_ke
 #pragma unroll
           for (int r = 0; r < 16; ++r) {
             const int x = 32 * kt + 8 * (r >> 2) + (r & 3);
-            sx[kt][r] = x <= hi && (x >= lo || x < sk) ? sx[kt][r] : -INFINITY;
+            sx[kt][r] = (x <= hi) & ((x >= lo) | (x < sk)) ? sx[kt][r] : -INFINITY;  // (no branches)
           }
         return;
       }

@@ -1317,6 +1317,9 @@ int64_t flash_window_splits(const WindowParams& p, int E, bool bf16) { return bf
 
 int flash_window_bf16_launch(const WindowParams& p, int E, hipStream_t stream) {
   if (!window_fits(p, E, 2)) return CA_DECLINED;
+  // Few keys: one wave per 32 rows with every key in registers, as flash_plan (whose
+  // strides' bound 256 keys meet by window_fits).
+  if (small_route(p.batch, p.seq_q, p.seq_k, p.heads, E, true)) return flash_window_small_launch(p, E, stream);
   switch (E) {
     case 32: return win_launch<32>(p, stream);
     case 64: return win_launch<64>(p, stream);

@@ -344,6 +344,7 @@ int flash_small_launch(const FlashParams& p, const FlashPlan& plan, int head_dim
 // The prefill with a window and sinks: splits of the keys (1: no workspace), and launch.
 int64_t flash_window_splits(const WindowParams& p, int head_dim, bool bf16);
 int flash_window_bf16_launch(const WindowParams& p, int head_dim, hipStream_t stream);
+int flash_window_small_launch(const WindowParams& p, int head_dim, hipStream_t stream);
 int flash_window_f32_launch(const WindowParams& p, int head_dim, hipStream_t stream);
 // Merges each row's `splits` partials (p.part_acc / p.part_ml) into p.out.
 int flash_combine_launch(const FlashParams& p, int head_dim, int bf16, int64_t splits, hipStream_t stream);

@@ -22,8 +22,14 @@
 // No barrier: the block is one wave.  Numerics are the reference's bf16 policy: fp32 logits,
 // p = 2^(s*c - max) with l summing the unrounded p, P rounded to bf16 for P.V,
 // the output rounded once; a row that sees no key is 0.
+//
+// Window calls (P = WindowParams) differ in the mask, and redo rows that come out not
+// finite key by key (win_redo_row).
+#include <type_traits>
+
 #include "ca_device.h"
 #include "ca_internal.h"
+#include "ca_window.h"
 
 namespace ca {
 
@@ -81,8 +87,9 @@ __device__ __forceinline__ bf16x8 small_v_operand(const uint16_t* vs, int lane, 
   return bf16x8{a[0][0], a[0][1], a[0][2], a[0][3], a[1][0], a[1][1], a[1][2], a[1][3]};
 }
 
-template <int E, int NKB>
-__global__ __launch_bounds__(64) void flash_small_kernel(FlashParams p) {
+template <int E, int NKB, class P = FlashParams>
+__global__ __launch_bounds__(64) void flash_small_kernel(P p) {
+  constexpr bool WIN = std::is_same<P, WindowParams>::value;
   constexpr int NKS = E / 16;  // 16-dim steps of S
   constexpr int NDB = E / 32;  // 32-dim blocks of O
   const int lane = threadIdx.x, n = lane & 31, hf = lane >> 5;
@@ -142,12 +149,20 @@ __global__ __launch_bounds__(64) void flash_small_kernel(FlashParams p) {
 
   // Softmax of the row (base 2, scaled logits), masked to the row's keys.
   const int kend = live ? small_kend(p, row) : 0;
+  int hi = 0, lo = 0, sk = 0;  // WIN: the row's last key, its window's first, the sinks
+  if constexpr (WIN) {
+    hi = live ? imin(S - 1, row + S - L + p.right) : -1;
+    lo = imax(0, row + S - L - p.left);
+    sk = p.sinks;
+  }
   float m = -INFINITY;
 #pragma unroll
   for (int kb = 0; kb < NKB; ++kb)
 #pragma unroll
     for (int r = 0; r < 16; ++r) {
-      const float x = 32 * kb + small_acc_row(r, hf) < kend ? s[kb][r] * p.c : -INFINITY;
+      const int j = 32 * kb + small_acc_row(r, hf);
+      const bool seen = WIN ? (j <= hi) & ((j >= lo) | (j < sk)) : j < kend;
+      const float x = seen ? s[kb][r] * p.c : -INFINITY;
       s[kb][r] = x;
       m = fmaxf(m, x);
     }
@@ -175,6 +190,7 @@ __global__ __launch_bounds__(64) void flash_small_kernel(FlashParams p) {
   wave_lds_sync();  // the staged V rows before the transposed reads
   const float inv = l > 0.f ? 1.f / l : 0.f;
   uint16_t* out = static_cast<uint16_t*>(p.out) + ((w.b * L + row) * p.heads + w.h) * (int64_t)E;
+  bool bad = WIN && !(l < INFINITY);
 #pragma unroll
   for (int db = 0; db < NDB; ++db) {
     f32x16 o = {};
@@ -184,6 +200,10 @@ __global__ __launch_bounds__(64) void flash_small_kernel(FlashParams p) {
       for (int u = 0; u < 2; ++u)
         o = __builtin_amdgcn_mfma_f32_32x32x16_bf16(small_v_operand<E>(vs, lane, 2 * kb + u, db), pk[kb][u], o, 0, 0,
                                                     0);
+    if constexpr (WIN) {
+#pragma unroll
+      for (int r = 0; r < 16; ++r) bad |= !(fabsf(o[r]) < INFINITY);
+    }
     if (live) {
 #pragma unroll
       for (int i = 0; i < 4; ++i)
@@ -191,20 +211,37 @@ __global__ __launch_bounds__(64) void flash_small_kernel(FlashParams p) {
             u32x2{pack_bf16x2(o[4 * i] * inv, o[4 * i + 1] * inv), pack_bf16x2(o[4 * i + 2] * inv, o[4 * i + 3] * inv)};
     }
   }
+  if constexpr (WIN) {
+    const uint64_t bits = __ballot(bad && live);
+    uint32_t redo = (uint32_t)bits | (uint32_t)(bits >> 32);
+    if (__builtin_expect(redo == 0, 1)) return;
+    __builtin_amdgcn_fence(__ATOMIC_RELEASE, "workgroup");
+    __builtin_amdgcn_wave_barrier();
+    __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "workgroup");
+    const WinTiles all{0, 0, (S + 63) / 64};
+    uint16_t* ob = static_cast<uint16_t*>(p.out) + (w.b * L * p.heads + w.h) * (int64_t)E;
+    while (redo) {
+      const int r = w.r0 + __builtin_ctz(redo);
+      redo &= redo - 1;
+      win_redo_row<E, uint16_t, 64>(p, all, 0, all.n, qp, kp, vp, r, [&](float, float rl, int d, float a) {
+        ob[(int64_t)r * p.heads * E + d] = (uint16_t)pack_bf16x2(rl != 0.f ? a / rl : 0.f, 0.f);
+      });
+    }
+  }
 }
 
-template <int E>
-static int small_launch_t(const FlashParams& p, const FlashPlan& plan, hipStream_t stream) {
+template <int E, class P>
+static int small_launch_t(const P& p, const FlashPlan& plan, hipStream_t stream) {
   const dim3 grid((unsigned)plan.gx), block(64);
   switch (cdiv(p.seq_k, 32)) {
-    case 1: hipLaunchKernelGGL((flash_small_kernel<E, 1>), grid, block, 0, stream, p); break;
-    case 2: hipLaunchKernelGGL((flash_small_kernel<E, 2>), grid, block, 0, stream, p); break;
-    case 3: hipLaunchKernelGGL((flash_small_kernel<E, 3>), grid, block, 0, stream, p); break;
-    case 4: hipLaunchKernelGGL((flash_small_kernel<E, 4>), grid, block, 0, stream, p); break;
-    case 5: hipLaunchKernelGGL((flash_small_kernel<E, 5>), grid, block, 0, stream, p); break;
-    case 6: hipLaunchKernelGGL((flash_small_kernel<E, 6>), grid, block, 0, stream, p); break;
-    case 7: hipLaunchKernelGGL((flash_small_kernel<E, 7>), grid, block, 0, stream, p); break;
-    case 8: hipLaunchKernelGGL((flash_small_kernel<E, 8>), grid, block, 0, stream, p); break;
+    case 1: hipLaunchKernelGGL((flash_small_kernel<E, 1, P>), grid, block, 0, stream, p); break;
+    case 2: hipLaunchKernelGGL((flash_small_kernel<E, 2, P>), grid, block, 0, stream, p); break;
+    case 3: hipLaunchKernelGGL((flash_small_kernel<E, 3, P>), grid, block, 0, stream, p); break;
+    case 4: hipLaunchKernelGGL((flash_small_kernel<E, 4, P>), grid, block, 0, stream, p); break;
+    case 5: hipLaunchKernelGGL((flash_small_kernel<E, 5, P>), grid, block, 0, stream, p); break;
+    case 6: hipLaunchKernelGGL((flash_small_kernel<E, 6, P>), grid, block, 0, stream, p); break;
+    case 7: hipLaunchKernelGGL((flash_small_kernel<E, 7, P>), grid, block, 0, stream, p); break;
+    case 8: hipLaunchKernelGGL((flash_small_kernel<E, 8, P>), grid, block, 0, stream, p); break;
     default: return CA_DECLINED;
   }
   return ca_launch_status();
@@ -219,13 +256,23 @@ FlashPlan small_plan(const FlashParams& p) {
   return plan;
 }
 
-int flash_small_launch(const FlashParams& p, const FlashPlan& plan, int E, hipStream_t stream) {
+template <class P>
+static int small_launch(const P& p, const FlashPlan& plan, int E, hipStream_t stream) {
   switch (E) {
     case 32: return small_launch_t<32>(p, plan, stream);
     case 64: return small_launch_t<64>(p, plan, stream);
     case 128: return small_launch_t<128>(p, plan, stream);
   }
   return CA_DECLINED;
+}
+
+int flash_small_launch(const FlashParams& p, const FlashPlan& plan, int E, hipStream_t stream) {
+  return small_launch(p, plan, E, stream);
+}
+
+int flash_window_small_launch(const WindowParams& p, int E, hipStream_t stream) {
+  const FlashPlan plan = small_plan(p);
+  return plan.kind == kPlanSmall ? small_launch(p, plan, E, stream) : CA_DECLINED;
 }
 
 }  // namespace ca
