@@ -32,10 +32,11 @@
 // walks about the same number of tiles.
 //
 // Window calls (P = WindowParams, ca_window.h): the block's keys are a list of tiles, the
-// sinks' and the window's, each masked by the rows' own limits.  A row's first tile may
-// hold nothing that it sees, or a few sinks far above or below the window's logits, so
-// there is no fixed max to take from it: these calls run the walk with the running max.
-// Rows that come out not finite are redone key by key (win_redo_row).
+// sinks' and the window's, each masked by the rows' own limits.  A row's fixed max is taken
+// from the first tile that shows it a finite logit, which may be a later one than its
+// neighbours' (KG = 2: a group's own, so the groups' sums are levelled before they merge);
+// the safe walk is the same.  Rows that come out not finite are redone key by key
+// (win_redo_row).
 #pragma once
 
 namespace ca {
@@ -397,6 +398,15 @@ __global__ __launch_bounds__(256 * KG, (DuoCfg<E, KG>::WAVES)) void flash_duo_ke
       // their wait, and so a wait for the tile loads after them, into every iteration).
 #pragma unroll
       for (int s = 0; s < NS; ++s) asm volatile("" : "+v"(qr[s]));
+      // WIN, fast walk: some row has not seen a finite logit yet.  Such a row's max is fixed
+      // at the first tile that shows it one.
+      bool open = false;
+      auto fix_max = [&](const f32x16 (&sx)[2]) __attribute__((always_inline)) {
+        const float mx = row_max(sx);
+        m = m == -INFINITY ? mx + kMaxLift : m;
+        nmu = m == -INFINITY ? 0.f : -m;
+        open = __any(m == -INFINITY);
+      };
       f32x16 st[2][2];           // S^T of two consecutive tiles: [parity][32-key half]
       uint32_t kb = kl, vb = 0;  // this lane's K base of the next S tile, V offset of this tile
 
@@ -420,6 +430,8 @@ __global__ __launch_bounds__(256 * KG, (DuoCfg<E, KG>::WAVES)) void flash_duo_ke
             m = mn;
             nmu = mn == -INFINITY ? 0.f : -mn;
           }
+        } else if (WIN && open) {
+          fix_max(st[PAR]);
         }
         bf16x8 op[SEQ.n];
         auto read = [&](int i) __attribute__((always_inline)) {
@@ -477,7 +489,7 @@ __global__ __launch_bounds__(256 * KG, (DuoCfg<E, KG>::WAVES)) void flash_duo_ke
         };
         if (KG == 2) {
           if (nkt_w > 0) first();
-          if (!safe) {  // group 0's max for both (a wave without a tile there has none here)
+          if (!WIN && !safe) {  // group 0's max for both (a wave without a tile there has none here)
             float* fixed = reinterpret_cast<float*>(duo_smem + C::TILES) + 32 * wv + li;
             if (grp == 0) *fixed = m;
             __syncthreads();
@@ -489,7 +501,10 @@ __global__ __launch_bounds__(256 * KG, (DuoCfg<E, KG>::WAVES)) void flash_duo_ke
           nmu = m == -INFINITY ? 0.f : -m;
           // No finite logit among the first tile's visible keys: the max would be fixed
           // at 0, and p of later logits far below 0 flush.
-          if (!safe) fine = m != -INFINITY || (p.causal && kbeg > r0 + li + diag);
+          if (WIN)
+            open = __any(m == -INFINITY);
+          else if (!safe)
+            fine = m != -INFINITY || (p.causal && kbeg > r0 + li + diag);
           for (; t + 1 < nkt_w; t += 2) {
             body(std::integral_constant<int, 0>{}, t);
             body(std::integral_constant<int, 1>{}, t + 1);
@@ -511,13 +526,8 @@ __global__ __launch_bounds__(256 * KG, (DuoCfg<E, KG>::WAVES)) void flash_duo_ke
 
     // One loop body serves both walks; the block takes the second where a wave failed.
     bool safe = false;
-    if constexpr (WIN) {
-      walk(true);
-      __syncthreads();  // the tile buffers are free
-      safe = true;
-    }
 #pragma unroll 1
-    while (!WIN) {
+    for (;;) {
       const bool fine = walk(safe);
       __syncthreads();  // the tile buffers are free
       if (safe) break;
@@ -532,6 +542,14 @@ __global__ __launch_bounds__(256 * KG, (DuoCfg<E, KG>::WAVES)) void flash_duo_ke
     }
 
     char* stage = duo_smem + wv * (KG == 2 ? C::MERGE : 32 * C::STAGE_ROW);
+    if constexpr (KG == 2 && WIN) {
+      // The groups' fixed maxima are their own: the sums' sizes go into them before the merge.
+      float lt = l + __shfl_xor(l, 32);
+      const float f = level_partial(m, lt);
+      l *= f;
+#pragma unroll
+      for (int d = 0; d < ND; ++d) o[d] *= f;
+    }
     if constexpr (KG == 2) {
       // Group 1's sums go through LDS to group 0, which merges and stores.
       float* mb = reinterpret_cast<float*>(stage) + lane;
