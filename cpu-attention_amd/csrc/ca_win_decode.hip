@@ -73,6 +73,29 @@ __device__ __forceinline__ uint32_t low_bits(int64_t n) {
   return n <= 0 ? 0u : (n >= kUnit ? 0xffffu : (1u << (int)n) - 1u);
 }
 
+// The sums of v[0 .. N) over the lanes that differ in the bits FIRST, 2 FIRST, .. 32 of their
+// number.  At each bit a lane passes half of its values on and adds the other half of its
+// neighbour's (N - 1 exchanges instead of N times the bits): it ends with the sums of
+// v[at ..), max(1, N FIRST / 64) of them in v[0 ..), and returns at.
+template <int N, int FIRST, int A>
+__device__ __forceinline__ int fold_lanes(float (&v)[A], int lane) {
+  if constexpr (FIRST >= kWave) {
+    return 0;
+  } else if constexpr (N > 1) {
+    constexpr int H = N / 2;
+    const bool up = lane & FIRST;
+#pragma unroll
+    for (int i = 0; i < H; ++i) {
+      const float lo = v[i], hi = v[H + i];
+      v[i] = (up ? hi : lo) + __shfl_xor(up ? lo : hi, FIRST);
+    }
+    return (up ? H : 0) + fold_lanes<H, 2 * FIRST>(v, lane);
+  } else {
+    v[0] += __shfl_xor(v[0], FIRST);
+    return fold_lanes<1, 2 * FIRST>(v, lane);
+  }
+}
+
 template <int E, bool BF, bool F8>
 struct WinShape {
   static constexpr int CES = F8 ? 1 : (BF ? 2 : 4);  // bytes of a cache element
@@ -90,7 +113,7 @@ __device__ __forceinline__ void win_tile(const WinDecodeParams& p, const Span& s
   using D = WinShape<E, BF, F8>;
   constexpr int W = D::W, DPL = D::DPL, LPR = D::LPR, G = D::G, CES = D::CES;
   constexpr int NU = TK / kUnit, NQ = TK / 4, SPLIT = kWave / NQ, WPL = W / SPLIT;
-  static_assert(TK == 64, "one 64-bit mask of visible keys");
+  static_assert((TK == 64 || TK == 128) && W % SPLIT == 0, "tile shape");
   const int lane = threadIdx.x & 63;
   const int quad = lane % NQ, phase = lane / NQ;  // key quad of the tile, words phase, phase + SPLIT, ...
 
@@ -140,9 +163,10 @@ __device__ __forceinline__ void win_tile(const WinDecodeParams& p, const Span& s
       }
     }
   }
-  uint64_t mask = 0;
+  uint64_t mask[TK / 64] = {};  // the tile's visible keys
 #pragma unroll
-  for (int u = 0; u < NU; ++u) mask |= (uint64_t)(uint32_t)__builtin_amdgcn_readlane((int)vis, u) << (kUnit * u);
+  for (int u = 0; u < NU; ++u)
+    mask[u / 4] |= (uint64_t)(uint32_t)__builtin_amdgcn_readlane((int)vis, u) << (kUnit * (u % 4));
 
   // The new token of a 16- or 32-bit cache: its words and q's, and its key in the tile.  Its
   // logit comes from these registers and its V row from where it lies, so nothing waits
@@ -187,13 +211,13 @@ __device__ __forceinline__ void win_tile(const WinDecodeParams& p, const Span& s
       const int64_t vu = __shfl(vb, key / kUnit);
       const char* at = reinterpret_cast<const char*>(p.vc) + (vu + (int64_t)(key & (kUnit - 1)) * E) * CES;
       if (APPEND && !F8 && key == newj) at = vnew;
-      if (mask >> key & 1) v4[i] = __builtin_nontemporal_load(reinterpret_cast<const u32x4*>(at + dl * 16));
+      if (mask[G * (b0 + i) / 64] >> (key % 64) & 1) v4[i] = __builtin_nontemporal_load(reinterpret_cast<const u32x4*>(at + dl * 16));
     }
   };
 
   // ---- Q.K
   float s[4] = {0.f, 0.f, 0.f, 0.f};
-  const uint32_t qvis = (uint32_t)(mask >> (4 * quad)) & 15u;
+  const uint32_t qvis = (uint32_t)(mask[TK == 64 || quad < 16 ? 0 : 1] >> (4 * (quad % 16))) & 15u;
   const int64_t kbu = __shfl(kb, quad >> 2);
   float cs = p.c;
   if (F8) cs *= __shfl(ksc, quad >> 2);
@@ -268,35 +292,36 @@ __device__ __forceinline__ void win_tile(const WinDecodeParams& p, const Span& s
       lnew = wave_sum(lnew);
     }
   }
-  // The SPLIT lanes of a quad sum their parts.  Scaled logits: -inf for a masked key,
-  // +inf for a NaN (its row comes out NaN then; as a NaN, the maxima would skip it and
-  // a tile of nothing else would count as empty).
-  float x[4], mx = -INFINITY;
+  // The SPLIT lanes of a quad sum their parts, each ending with the logits of KPL of its keys,
+  // 4 quad + j0 ...  Scaled logits: -inf for a masked key, +inf for a NaN (its row comes out
+  // NaN then; as a NaN, the maxima would skip it and a tile of nothing else would count as
+  // empty).
+  constexpr int KPL = 4 / SPLIT;
+  const int j0 = fold_lanes<4, NQ>(s, lane);
+  float x[KPL], mx = -INFINITY;
 #pragma unroll
-  for (int j = 0; j < 4; ++j) {
-#pragma unroll
-    for (int o = NQ; o < kWave; o <<= 1) s[j] += __shfl_xor(s[j], o);
-    if (APPEND && !F8 && 4 * quad + j == newj) s[j] = lnew;
+  for (int j = 0; j < KPL; ++j) {
+    if (APPEND && !F8 && 4 * quad + j0 + j == newj) s[j] = lnew;
     x[j] = s[j] * cs;
     x[j] = x[j] != x[j] ? INFINITY : x[j];
-    x[j] = qvis >> j & 1 ? x[j] : -INFINITY;
+    x[j] = qvis >> (j0 + j) & 1 ? x[j] : -INFINITY;
     mx = fmaxf(mx, x[j]);
   }
   const float m = wave_max(mx), mu = m == -INFINITY ? 0.f : m;
-  float pr[4], ls = 0.f;
+  float pr[KPL], ls = 0.f;
 #pragma unroll
-  for (int j = 0; j < 4; ++j) {
+  for (int j = 0; j < KPL; ++j) {
     pr[j] = __builtin_amdgcn_exp2f(x[j] - mu);
     ls += pr[j];
   }
-  const float l = wave_sum(phase == 0 ? ls : 0.f);  // one lane per quad counts it
+  const float l = wave_sum(ls);
   if (F8) {
     const float vq = __shfl(vsc, quad >> 2);
 #pragma unroll
-    for (int j = 0; j < 4; ++j) pr[j] *= vq;
+    for (int j = 0; j < KPL; ++j) pr[j] *= vq;
   }
-  wave_lds_sync();
-  if (phase == 0) *reinterpret_cast<f32x4*>(&p_lds[4 * quad]) = f32x4{pr[0], pr[1], pr[2], pr[3]};
+#pragma unroll
+  for (int j = 0; j < KPL; ++j) p_lds[4 * quad + j0 + j] = pr[j];
   wave_lds_sync();
 
   // ---- P.V
@@ -308,7 +333,7 @@ __device__ __forceinline__ void win_tile(const WinDecodeParams& p, const Span& s
     if (!EARLY) load_v(b0);
 #pragma unroll
     for (int i = 0; i < B; ++i) {
-      if (mask >> (g + G * (b0 + i)) & 1) {
+      if (mask[G * (b0 + i) / 64] >> ((g + G * (b0 + i)) % 64) & 1) {
         const float pj = p_lds[g + G * (b0 + i)];
 #pragma unroll
         for (int x4 = 0; x4 < 4; ++x4) {
@@ -329,14 +354,12 @@ __device__ __forceinline__ void win_tile(const WinDecodeParams& p, const Span& s
       }
     }
   }
+  // The lane groups sum theirs: a lane ends with NP dims of its 16 bytes (the same ones as
+  // another lane's, where the groups outnumber the dims).
+  constexpr int NP = DPL > G ? DPL / G : 1;
+  const int d0 = dl * DPL + fold_lanes<DPL, LPR>(acc, lane);
 #pragma unroll
-  for (int o = LPR; o < kWave; o <<= 1)
-#pragma unroll
-    for (int i = 0; i < DPL; ++i) acc[i] += __shfl_xor(acc[i], o);
-  if (lane < LPR) {
-#pragma unroll
-    for (int i = 0; i < DPL; ++i) part[lane * DPL + i] = acc[i];
-  }
+  for (int i = 0; i < NP; ++i) part[d0 + i] = acc[i];
   if (lane == 0) {
     part[E] = m;
     part[E + 1] = l;
