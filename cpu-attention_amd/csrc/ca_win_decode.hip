@@ -25,11 +25,11 @@ namespace ca {
 
 constexpr int kUnit = 16;     // keys per unit: never straddles a page
 constexpr int kWinTile = 64;  // keys per tile
-// V rows of a lane up to which they are loaded before the logits.  4 (8-bit E = 32 and 64,
-// bf16 E = 32) hide a load's latency for few registers (8-bit fp32 N=8 H=16 E=64 14.1 -> 13.1
-// us); 8 take 8-bit E = 128 to 129 registers and one block per CU (N=64 H=32, lengths to
-// 4095: 193 -> 284 us), 16 bf16 E = 64 the same way (52 -> 61 us).
-constexpr int kEarlyRows = 4;
+// V rows of a lane up to which they are loaded before the logits: 2 (8-bit E = 32) hide a
+// load's latency for few registers.  4 take 8-bit E = 64 from 80 to 99 registers, two blocks
+// per CU instead of three (N=64 H=32, lengths to 4095: 107 -> 136 us), 8 leave 8-bit E = 128
+// one (193 -> 284 us).
+constexpr int kEarlyRows = 2;
 
 // Positions and pages fit 32 unsigned bits (lengths are 32-bit, plus at most 2^30 new
 // tokens; the launcher bounds the page), and a 32-bit division takes a third of a 64-bit one.
