@@ -26,7 +26,7 @@ namespace ca {
 constexpr int kUnit = 16;     // keys per unit: never straddles a page
 constexpr int kWinTile = 64;  // keys per tile
 // V rows of a lane up to which they are loaded before the logits: 2 (8-bit E = 32) hide a
-// load's latency for few registers.  4 take 8-bit E = 64 from 80 to 99 registers, two blocks
+// load's latency for few registers.  4 take 8-bit E = 64 from 64 to 99 registers, two blocks
 // per CU instead of three (N=64 H=32, lengths to 4095: 107 -> 136 us), 8 leave 8-bit E = 128
 // one (193 -> 284 us).
 constexpr int kEarlyRows = 2;

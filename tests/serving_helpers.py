@@ -27,7 +27,7 @@ class Paged:
     """Sequences in a paged cache written here, token by token, in the cache's layout: pages
     in random order, everything else NaN, and the table's unused entries out of range."""
 
-    def __init__(self, lens, heads, dim, page, dtype, seed, device, fp8=False, spare=0, k_scale=1.0):
+    def __init__(self, lens, heads, dim, page, dtype, seed, device, fp8=False, spare=0):
         g = torch.Generator().manual_seed(seed)
         self.lens, self.page, self.heads, self.dim, self.dtype = list(lens), page, heads, dim, dtype
         need = [-(-(n + spare) // page) for n in lens]
@@ -42,7 +42,7 @@ class Paged:
         self.blocks = total
         self.lens_t = torch.tensor(self.lens, dtype=torch.int32, device=device)
         self.q = torch.randn(len(lens), 1, heads, dim, generator=g).to(dtype).to(device)
-        ks = [torch.randn(n, heads, dim, generator=g) * k_scale for n in lens]
+        ks = [torch.randn(n, heads, dim, generator=g) for n in lens]
         vs = [torch.randn(n, heads, dim, generator=g) for n in lens]
         if fp8:
             # codes and scales of every page; a page not in use holds NaN codes and a NaN scale
@@ -80,15 +80,15 @@ class Paged:
                 kc[blk, :, :part.stop - part.start] = ks[i][part].to(dtype).transpose(0, 1)
                 vc[blk, :, :part.stop - part.start] = vs[i][part].to(dtype).transpose(0, 1)
         per = 4 // kc.element_size()
-        self.kc = kc.view(total, heads, page, dim // per, per).transpose(2, 3).reshape(total, heads, page, dim).to(device)
+        self.kc = kc.view(total, heads, page, dim // per, per).transpose(2, 3).contiguous().view(total, heads, page, dim).to(device)
         self.vc = vc.to(device)
         self.ks = [values(x.to(dtype)) for x in ks]
         self.vs = [values(x.to(dtype)) for x in vs]
 
-    def rows_of(self, which=None):
+    def rows_of(self):
         """K as [blocks, heads, page, dim] rows (the layout undone) and V, on the CPU."""
         per = 4 // self.kc.element_size()
-        k = self.kc.cpu().view(torch.uint8).view(self.blocks, self.heads, self.dim // per, self.page, 4)
+        k = self.kc.cpu().contiguous().view(torch.uint8).view(self.blocks, self.heads, self.dim // per, self.page, 4)
         k = k.transpose(2, 3).reshape(self.blocks, self.heads, self.page, -1)
         return k, self.vc.cpu().view(torch.uint8)
 

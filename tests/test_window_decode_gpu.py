@@ -87,15 +87,34 @@ def test_against_float64(cuda, shape, dtype, fp8):
     close(out, ref, dtype)
 
 
+# (lengths, heads, dim, page, left, sinks, new tokens): one token is stored by the decode
+# itself up to 1024 rows and, in an 8-bit cache, pages of 64; by a kernel before it above,
+# and for more tokens
+APPENDS = [
+    ([0, 15, 16, 40, 700, 33], 3, 64, 16, 50, 2, 1),
+    ([0, 15, 16, 40, 700, 33], 3, 64, 16, 50, 2, 5),
+    ([0, 15, 16, 40, 700, 33], 3, 64, 16, 50, 2, 37),
+    ([0, 1, 31, 32, 33, 64, 65, 500], 2, 128, 32, 3, 0, 1),
+    ([47, 48, 49, 95, 96, 10, 0, 300], 2, 32, 48, 0, 0, 1),
+    ([63, 64, 100, 127, 128, 1000], 2, 64, 64, 20, 70, 1),    # sinks in the last page, or past it
+    ([10, 44, 45, 46, 63], 2, 64, 64, 0, 40, 1),
+    ([79, 80, 81, 200, 5], 2, 64, 80, 30, 3, 1),              # pages over 64
+    ([2050, 2047, 1023, 511, 512, 513], 1, 64, 16, -1, 0, 1),  # at the ends of blocks of tiles
+    ([2050, 575, 576, 577], 2, 128, 64, 559, 16, 1),
+    ([3 + i % 70 for i in range(350)], 3, 32, 16, 25, 1, 1),   # 1050 rows
+]
+
+
 @pytest.mark.parametrize("dtype,fp8", KINDS, ids=IDS)
-def test_append_of_one_and_of_many(cuda, dtype, fp8):
+@pytest.mark.parametrize("shape", APPENDS, ids=lambda s: f"{len(s[0])}x{s[0][0]}-" + "-".join(map(str, s[1:])))
+def test_append_of_one_and_of_many(cuda, shape, dtype, fp8):
     """New tokens are seen by the query; the cache holds them afterwards, bit for bit, and
     nothing else changes (8-bit: by the store's rule)."""
-    lens, h, d, page = [0, 15, 16, 40, 700, 33], 3, 64, 16
-    for n in (1, 5, 37):
+    lens, h, d, page, left, sinks, n = shape
+    for size in (1.0, 300.0) if n == 1 and len(lens) < 100 else (1.0,):  # 300: every 8-bit page is rescaled
         p = Paged(lens, h, d, page, dtype, n, cuda, fp8=fp8, spare=n)
         g = torch.Generator().manual_seed(n)
-        fused = torch.randn(len(lens), n, 2, h, d, generator=g).to(dtype).to(cuda)
+        fused = (torch.randn(len(lens), n, 2, h, d, generator=g) * size).to(dtype).to(cuda)
         k, v = fused[:, :, 0], fused[:, :, 1]
         slots = [int(p.table[i, (s + j) // page]) * page + (s + j) % page for i, s in enumerate(lens) for j in range(n)]
         kr, vr = values(k).reshape(-1, h, d), values(v).reshape(-1, h, d)
@@ -104,17 +123,21 @@ def test_append_of_one_and_of_many(cuda, dtype, fp8):
             for s in (want.scales[0], want.scales[1]):
                 s[np.isnan(s)] = 0.0
             want.store(kr, vr, slots)
-            seq = lambda i, w: np.concatenate([want.values(w)[int(b)].transpose(1, 0, 2) for b in p.table[i, :-(-(lens[i] + n) // page)]])  # noqa: E731
-            p.ks, p.vs = ([seq(i, w)[:lens[i] + n] for i in range(len(lens))] for w in (0, 1))
+
+            def seq(i, w):
+                pages = p.table[i, :-(-(lens[i] + n) // page)]
+                return np.concatenate([want.values(w)[int(b)].transpose(1, 0, 2) for b in pages])[:lens[i] + n]
+
+            p.ks, p.vs = ([seq(i, w) for i in range(len(lens))] for w in (0, 1))
         else:
             k0, v0 = p.rows_of()
             p.ks = [np.concatenate([x, kr[i * n:(i + 1) * n]]) for i, x in enumerate(p.ks)]
             p.vs = [np.concatenate([x, vr[i * n:(i + 1) * n]]) for i, x in enumerate(p.vs)]
-        out = call(p, fp8, k=k, v=v, window_size=(50, -1), sink_tokens=2)
+        out = call(p, fp8, k=k, v=v, window_size=(left, -1), sink_tokens=sinks)
         k1, v1 = p.rows_of()
         if fp8:
-            same = lambda a, b: np.array_equal(R.e4m3_decode(a.numpy()), R.e4m3_decode(b), equal_nan=True)  # noqa: E731
-            assert same(k1, want.codes[0]) and same(v1, want.codes[1])
+            for got, ref in ((k1, want.codes[0]), (v1, want.codes[1])):
+                assert np.array_equal(R.e4m3_decode(got.numpy()), R.e4m3_decode(ref), equal_nan=True)
             for got, w in ((p.kscale, want.scales[0]), (p.vscale, want.scales[1])):
                 got = got.cpu().numpy()
                 assert np.array_equal(got[~np.isnan(got)], w[~np.isnan(got)])
@@ -125,7 +148,7 @@ def test_append_of_one_and_of_many(cuda, dtype, fp8):
                 for s, row in zip(slots, rows):
                     was[s // page, :, s % page] = row.view(h, d * es)
                 assert torch.equal(now, was)
-        close(out, R.decode(values(p.q)[:, 0], p.ks, p.vs, d ** -0.5, 50, 2), dtype)
+        close(out, R.decode(values(p.q)[:, 0], p.ks, p.vs, d ** -0.5, left, sinks), dtype)
 
 
 @pytest.mark.parametrize("dtype,fp8", KINDS, ids=IDS)
