@@ -327,6 +327,10 @@ static WindowParams window_params(const FlashParams& f, const WindowSides& w) {
   return p;
 }
 
+static int64_t window_splits(const WindowParams& p, int64_t head_dim, int32_t dtype) {
+  return dtype == CA_BF16 ? flash_window_bf16_splits(p) : flash_window_f32_splits(p, (int)head_dim);
+}
+
 extern "C" int64_t ca_flash_window_workspace_bytes(int64_t batch, int64_t seq_q, int64_t seq_k, int64_t num_heads,
                                                    int64_t head_dim, int32_t dtype, int32_t causal, int64_t left,
                                                    int64_t right, int64_t sinks) {
@@ -339,7 +343,7 @@ extern "C" int64_t ca_flash_window_workspace_bytes(int64_t batch, int64_t seq_q,
   f.seq_q = seq_q;
   f.seq_k = seq_k;
   f.heads = num_heads;
-  const int64_t splits = flash_window_splits(window_params(f, w), (int)head_dim, dtype == CA_BF16);
+  const int64_t splits = window_splits(window_params(f, w), head_dim, dtype);
   return splits > 1 ? batch * num_heads * seq_q * splits * (head_dim + 2) * 4 : 0;
 }
 
@@ -377,7 +381,7 @@ extern "C" int ca_flash_window(const ca_flash_window_args* wa, void* stream) {
   }
   f.c = a->scale * kLog2e;
   WindowParams p = window_params(f, w);
-  const int64_t splits = flash_window_splits(p, (int)a->head_dim, a->dtype == CA_BF16);
+  const int64_t splits = window_splits(p, a->head_dim, a->dtype);
   if (splits > 1) {
     const int64_t slots = a->batch * a->num_heads * a->seq_q * splits;
     if (!a->workspace || !aligned16(a->workspace) || a->workspace_bytes < slots * (a->head_dim + 2) * 4) return CA_DECLINED;

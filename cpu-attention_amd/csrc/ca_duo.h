@@ -657,7 +657,8 @@ __global__ __launch_bounds__(256 * KG, (DuoCfg<E, KG>::WAVES)) void flash_duo_ke
   }
 }
 
-// How a window call runs: kg key groups and the splits of its blocks' tiles (1: none).
+// How a window call runs: kg key groups and the splits of its blocks' tiles (1: none), by
+// duo_plan's lines with T the most tiles that a block walks.
 struct WinPlan {
   int kg;
   int64_t items, splits;
@@ -666,7 +667,11 @@ inline WinPlan win_plan(const WindowParams& p) {
   constexpr int BM = DuoCfg<64, 1>::BM, BN = DuoCfg<64, 1>::BN;
   WinPlan w{1, p.batch * p.heads * cdiv(p.seq_q, BM), 1};
   const int64_t T = win_most_tiles(p, BM, BN);
-  if (w.items <= 64 && T >= 16) w.splits = 256 / w.items < T / 4 ? 256 / w.items : T / 4;
+  if (w.items <= 64 ? T >= 16 : (w.items <= 85 ? T >= 32 : w.items <= 170 && T >= 40)) {
+    w.splits = (w.items > 85 || (w.items > 64 && T >= 96) ? 512 : 256) / w.items;
+    w.splits = w.splits < T / 4 ? w.splits : T / 4;
+    w.splits = w.splits < kTiledMaxSplits ? w.splits : kTiledMaxSplits;  // what the combine merges
+  }
   if (w.splits <= 1 && w.items <= 256 && T > 8) w.kg = 2;
   return w;
 }

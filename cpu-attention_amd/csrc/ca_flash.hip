@@ -1313,7 +1313,7 @@ int flash_launch(const FlashParams& p, int E, int bf16, hipStream_t stream) {
   return CA_DECLINED;
 }
 
-int64_t flash_window_splits(const WindowParams& p, int E, bool bf16) { return bf16 ? win_plan(p).splits : 1; }
+int64_t flash_window_bf16_splits(const WindowParams& p) { return win_plan(p).splits; }
 
 int flash_window_bf16_launch(const WindowParams& p, int E, hipStream_t stream) {
   if (!window_fits(p, E, 2)) return CA_DECLINED;

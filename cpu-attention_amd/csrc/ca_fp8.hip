@@ -75,8 +75,8 @@ __global__ __launch_bounds__(64 * kStore8Waves) void store8_scan_kernel(Store8Pa
   __syncthreads();
   bool earlier = false;
   for (int64_t j = threadIdx.x; j < p.ntok; j += 64 * kStore8Waves) {
-    const int64_t t = p.slots[j] - blk * p.page;
-    if (t >= 0 && t < p.page) {
+    const uint64_t t = (uint64_t)p.slots[j] - (uint64_t)(blk * p.page);
+    if (t < (uint64_t)p.page) {
       earlier |= j < i;
       atomicMax(&owner[t], (int)j);
     }

@@ -342,7 +342,8 @@ FlashPlan rows_plan(const FlashParams& p, int head_dim, bool bf16);
 FlashPlan small_plan(const FlashParams& p);
 int flash_small_launch(const FlashParams& p, const FlashPlan& plan, int head_dim, hipStream_t stream);
 // The prefill with a window and sinks: splits of the keys (1: no workspace), and launch.
-int64_t flash_window_splits(const WindowParams& p, int head_dim, bool bf16);
+int64_t flash_window_bf16_splits(const WindowParams& p);
+int64_t flash_window_f32_splits(const WindowParams& p, int head_dim);
 int flash_window_bf16_launch(const WindowParams& p, int head_dim, hipStream_t stream);
 int flash_window_small_launch(const WindowParams& p, int head_dim, hipStream_t stream);
 int flash_window_f32_launch(const WindowParams& p, int head_dim, hipStream_t stream);

@@ -14,6 +14,9 @@
 // the same RB rows, each wave 32 of a tile's 128 keys, merged in LDS at the end: for calls
 // whose 128-row blocks leave CUs idle, four or (RB = 16) eight times the blocks.
 //
+// SPLIT: few rows over long windows; blockIdx.y takes a share of the tiles and leaves its
+// rows' partials (O, max, sum) for the combine kernel.
+//
 // Bound: the 32-bit MFMAs (157 TFLOP/s dense), either shape; masked parts of the window's
 // edge tiles are computed too.
 #include <type_traits>
@@ -37,7 +40,7 @@ struct WinF32Cfg {
   static_assert(CH * 1024 == BN * E, "tile shape");
 };
 
-template <int E, int KW, int RB>
+template <int E, int KW, int RB, bool SPLIT>
 __global__ __launch_bounds__(256, KW == 1 ? 2 : 1) void win_f32_kernel(WindowParams p) {
   using C = WinF32Cfg<E, KW, RB>;
   constexpr int BM = C::BM, BN = C::BN, RS = C::RS, CH = C::CH, NO = C::NO;
@@ -59,6 +62,9 @@ __global__ __launch_bounds__(256, KW == 1 ? 2 : 1) void win_f32_kernel(WindowPar
   const uint32_t* kg = reinterpret_cast<const uint32_t*>(p.k) + b * p.ks[0] + h * p.ks[2];
   const uint32_t* vg = reinterpret_cast<const uint32_t*>(p.v) + b * p.vs[0] + h * p.vs[2];
   const WinTiles wt = win_tiles(p, q0, BM, BN);
+  // The block's tiles [t0, t1) of the list.
+  const int share = SPLIT ? (wt.n + (int)gridDim.y - 1) / (int)gridDim.y : wt.n;
+  const int t0 = SPLIT ? imin((int)blockIdx.y * share, wt.n) : 0, t1 = imin(t0 + share, wt.n);
 
   // Chunk i of thread tid: key (tid + 256 i) / (E / 4) of the tile, dims 4 ((tid + 256 i) % (E / 4)).
   u32x4 kreg[CH], vreg[CH];
@@ -69,7 +75,7 @@ __global__ __launch_bounds__(256, KW == 1 ? 2 : 1) void win_f32_kernel(WindowPar
       const int c = tid + 256 * i, r = c / (E / 4), c4 = c % (E / 4);
       const int64_t key = k0 + r;
       kreg[i] = vreg[i] = u32x4{0, 0, 0, 0};
-      if (t < wt.n && key < S) {
+      if (t < t1 && key < S) {
         kreg[i] = *reinterpret_cast<const u32x4*>(kg + key * p.ks[1] + 4 * c4);
         vreg[i] = *reinterpret_cast<const u32x4*>(vg + key * p.vs[1] + 4 * c4);
       }
@@ -83,7 +89,7 @@ __global__ __launch_bounds__(256, KW == 1 ? 2 : 1) void win_f32_kernel(WindowPar
       *reinterpret_cast<u32x4*>(win_smem + (BN + r) * RS + 4 * c4) = vreg[i];
     }
   };
-  load_tile(0);
+  load_tile(t0);
 
   // Q: the lane's row, dims 4 NQ u + 4 qd + e in qr[4 u + e]: the dims that MFMA step 4 u + e
   // takes of each lane, of K's rows too.
@@ -109,7 +115,7 @@ __global__ __launch_bounds__(256, KW == 1 ? 2 : 1) void win_f32_kernel(WindowPar
   // Row of an RB x RB block that register r of the lane holds (its column is li), less 4 qd.
   auto acc_row = [](int r) { return 4 * NQ * (r >> 2) + (r & 3); };
   const int rhi = imin(S - 1, row + diag + p.right), rlo = imax(0, row + diag - p.left);
-  for (int t = 0; t < wt.n; ++t) {
+  for (int t = t0; t < t1; ++t) {
     store_tile();
     __syncthreads();
     load_tile(t + 1);
@@ -192,8 +198,16 @@ __global__ __launch_bounds__(256, KW == 1 ? 2 : 1) void win_f32_kernel(WindowPar
   float lt = l;
 #pragma unroll
   for (int w = RB; w < 64; w <<= 1) lt += __shfl_xor(lt, w);
-  const float inv = lt > 0.f ? 1.f / lt : 0.f;
-  float* out = reinterpret_cast<float*>(p.out) + (b * p.seq_q * p.heads + h) * E;
+  // Row r's output, or (SPLIT) its partial slot's unnormalised dims, max and sum.
+  const float inv = SPLIT ? 1.f : (lt > 0.f ? 1.f / lt : 0.f);
+  auto slot = [&](int r) { return ((b * p.heads + h) * p.seq_q + r) * gridDim.y + blockIdx.y; };
+  auto row_out = [&](int r) {
+    return SPLIT ? p.part_acc + slot(r) * E : reinterpret_cast<float*>(p.out) + ((b * p.seq_q + r) * p.heads + h) * E;
+  };
+  if (SPLIT && row < L && qd == 0) {
+    p.part_ml[2 * slot(row)] = m;
+    p.part_ml[2 * slot(row) + 1] = lt;
+  }
   bool bad = !(fabsf(lt) < INFINITY);
 #pragma unroll
   for (int d = 0; d < ND; ++d)
@@ -205,7 +219,7 @@ __global__ __launch_bounds__(256, KW == 1 ? 2 : 1) void win_f32_kernel(WindowPar
         bad |= !(fabsf(o[d][4 * g + j]) < INFINITY);
         x[j] = o[d][4 * g + j] * inv;
       }
-      if (row < L) *reinterpret_cast<f32x4*>(out + (int64_t)row * p.heads * E + RB * d + acc_row(4 * g) + 4 * qd) = x;
+      if (row < L) *reinterpret_cast<f32x4*>(row_out(row) + RB * d + acc_row(4 * g) + 4 * qd) = x;
     }
   const uint64_t bits = __ballot(bad);
   uint32_t redo = (uint32_t)bits | (uint32_t)(bits >> 32);
@@ -218,36 +232,68 @@ __global__ __launch_bounds__(256, KW == 1 ? 2 : 1) void win_f32_kernel(WindowPar
     const int r = r0 + __builtin_ctz(redo);
     redo &= redo - 1;
     if (r >= L) continue;
-    win_redo_row<E, uint32_t, BN>(p, wt, 0, wt.n, qg, kg, vg, r, [&](float rm, float rl, int d, float a) {
-      out[(int64_t)r * p.heads * E + d] = rl != 0.f ? a / rl : 0.f;
+    win_redo_row<E, uint32_t, BN>(p, wt, t0, t1, qg, kg, vg, r, [&](float rm, float rl, int d, float a) {
+      row_out(r)[d] = SPLIT ? a : (rl != 0.f ? a / rl : 0.f);
+      if (SPLIT && d == 0) {
+        p.part_ml[2 * slot(r)] = rm;
+        p.part_ml[2 * slot(r) + 1] = rl;
+      }
     });
   }
 }
 
-template <int E, int KW, int RB>
-static int win_f32_launch_t(const WindowParams& p, hipStream_t stream) {
-  using C = WinF32Cfg<E, KW, RB>;
-  const int64_t nb = p.batch * p.heads * cdiv(p.seq_q, C::BM);
-  if (nb > 0x7fffffff) return CA_DECLINED;
-  if (C::LDS_BYTES > 64 * 1024) {
-    const hipError_t e = hipFuncSetAttribute(reinterpret_cast<const void*>(win_f32_kernel<E, KW, RB>),
-                                             hipFuncAttributeMaxDynamicSharedMemorySize, C::LDS_BYTES);
-    if (e != hipSuccess) return CA_HIP_ERROR - (int)e;
-  }
-  hipLaunchKernelGGL((win_f32_kernel<E, KW, RB>), dim3((unsigned)nb), dim3(256), C::LDS_BYTES, stream, p);
-  return ca_launch_status();
-}
-
+// How a call runs: key waves and rows per wave of its blocks, and splits of their tiles.
 // 128-row blocks where they give every CU one (E = 128, whose 128-key tiles leave one block
 // per CU: nearly), else 32-row ones, else 16-row ones.  Measured (us, window 300 unless
 // noted, KW = 1 / KW = 4 RB = 32 / RB = 16): N=1 L=333 S=2500 window 512 H=12 E=64 67.5 /
 // 28.1 / 20.3; N=2 L=S=700 H=12 E=64 48.0 / 24.5 / 30.7; L=S=1536 H=16 E=64 48.6 / 43.7,
-// E=128 81.1 / 82.7; N=2 L=S=1024 H=16 E=128 81.8 / 102.
+// E=128 81.1 / 82.7; N=2 L=S=1024 H=16 E=128 81.8 / 102.  16-row blocks that leave half of the
+// CUs idle split lists of 4 tiles or more, at least kMinShare tiles each (L=64 H=8, unsplit /
+// shares of 4 / 2: E=64 window 2048 38 / 20.0 / 14.9, window 768 21.5 / 21.5 / 14.8, E=32
+// window 512 10.5 / 10.5 / 10.9).
+struct WinF32Plan {
+  int kw, rb;
+  int64_t blocks, splits;
+};
+constexpr int64_t kMinShare = 2;
+static WinF32Plan win_f32_plan(const WindowParams& p, int E) {
+  const int64_t bh = p.batch * p.heads;
+  WinF32Plan w{1, 32, bh * cdiv(p.seq_q, 128), 1};
+  if (w.blocks > (E == 128 ? 192 : 256)) return w;
+  w = WinF32Plan{4, 32, bh * cdiv(p.seq_q, 32), 1};
+  if (w.blocks > 256) return w;
+  w = WinF32Plan{4, 16, bh * cdiv(p.seq_q, 16), 1};
+  const int64_t T = win_most_tiles(p, 16, 128), by_tiles = T / kMinShare;
+  if (w.blocks > 0 && w.blocks <= 128 && by_tiles >= 2) w.splits = 256 / w.blocks < by_tiles ? 256 / w.blocks : by_tiles;
+  w.splits = w.splits < kTiledMaxSplits ? w.splits : kTiledMaxSplits;  // what the combine merges
+  return w;
+}
+
+int64_t flash_window_f32_splits(const WindowParams& p, int E) { return win_f32_plan(p, E).splits; }
+
+template <int E, int KW, int RB, bool SPLIT>
+static int win_f32_launch_t(const WindowParams& p, const WinF32Plan& w, hipStream_t stream) {
+  using C = WinF32Cfg<E, KW, RB>;
+  if (w.blocks > 0x7fffffff) return CA_DECLINED;
+  if (C::LDS_BYTES > 64 * 1024) {
+    const hipError_t e = hipFuncSetAttribute(reinterpret_cast<const void*>(win_f32_kernel<E, KW, RB, SPLIT>),
+                                             hipFuncAttributeMaxDynamicSharedMemorySize, C::LDS_BYTES);
+    if (e != hipSuccess) return CA_HIP_ERROR - (int)e;
+  }
+  hipLaunchKernelGGL((win_f32_kernel<E, KW, RB, SPLIT>), dim3((unsigned)w.blocks, (unsigned)w.splits), dim3(256),
+                     C::LDS_BYTES, stream, p);
+  return ca_launch_status();
+}
+
 template <int E>
 static int win_f32_launch_e(const WindowParams& p, hipStream_t stream) {
-  if (p.batch * p.heads * cdiv(p.seq_q, 128) > (E == 128 ? 192 : 256)) return win_f32_launch_t<E, 1, 32>(p, stream);
-  if (p.batch * p.heads * cdiv(p.seq_q, 32) > 256) return win_f32_launch_t<E, 4, 32>(p, stream);
-  return win_f32_launch_t<E, 4, 16>(p, stream);
+  const WinF32Plan w = win_f32_plan(p, E);
+  if (w.splits > 1) {
+    const int st = win_f32_launch_t<E, 4, 16, true>(p, w, stream);
+    return st == CA_OK ? flash_combine_launch(p, E, false, w.splits, stream) : st;
+  }
+  if (w.kw == 1) return win_f32_launch_t<E, 1, 32, false>(p, w, stream);
+  return w.rb == 32 ? win_f32_launch_t<E, 4, 32, false>(p, w, stream) : win_f32_launch_t<E, 4, 16, false>(p, w, stream);
 }
 
 int flash_window_f32_launch(const WindowParams& p, int E, hipStream_t stream) {

@@ -84,17 +84,19 @@ __host__ __device__ inline bool win_sees(const WindowParams& p, int pos, int j) 
 
 // Row `row` of (b, h) by one wave, key by key: what the matrix kernels leave to redo.  They
 // weigh a key that a row does not see with 0, and 0 times an infinity or a NaN in its V is
-// NaN; here such keys are not touched.  Rows that come out not finite are rare (or wrong
-// inputs), so this is plain: a lane takes a key of each tile for the logit and E / 64
-// dims (lanes below 32 for E = 32) for the sum.  T: 16-bit (bf16) or 32-bit (fp32) words.
-// Tiles [t0, t1) of the list, of BN keys; the scaled log2 max
-// m, sum l and the unnormalised dims go to `store(m, l, dim, acc)`.
+// NaN; here such keys are not touched.  Rows that come out not finite are rare, or the
+// inputs are wrong: a lane takes a key of each tile for the logit and E / 64 dims (lanes
+// below 32 for E = 32) for the sum, and a row whose every dim is NaN ends there (inputs of
+// NaNs would otherwise take this path over all of their keys).  T: 16-bit (bf16) or 32-bit
+// (fp32) words.  Tiles [t0, t1) of the list, of BN keys; the scaled log2 max m, sum l and
+// the unnormalised dims go to `store(m, l, dim, acc)`.
 template <int E, typename T, int BN, typename F>
 __device__ __forceinline__ void win_redo_row(const WindowParams& p, const WinTiles& w, int t0, int t1, const T* q,
                                              const T* k, const T* v, int row, F&& store) {
-  constexpr int DPC = E >= 64 ? E / 64 : 1;
+  constexpr int DPC = E >= 64 ? E / 64 : 1, PER = 16 / sizeof(T), AHEAD = 8;
   auto f32 = [](T x) { return __uint_as_float(sizeof(T) == 2 ? (uint32_t)x << 16 : (uint32_t)x); };
   const int lane = threadIdx.x & 63, S = (int)p.seq_k, pos = row + S - (int)p.seq_q;
+  const bool dims = lane * DPC < E;
   const T* qr = q + row * p.qs[1];
   float m = -INFINITY, l = 0.f, acc[DPC];
 #pragma unroll
@@ -108,8 +110,21 @@ __device__ __forceinline__ void win_redo_row(const WindowParams& p, const WinTil
       float x = -INFINITY;
       if (seen) {
         x = 0.f;
-#pragma unroll 1
-        for (int d = 0; d < E; ++d) x = fmaf(f32(k[j * p.ks[1] + d]), f32(qr[d]), x);
+#pragma unroll 4
+        for (int d = 0; d < E; d += PER) {  // 16 bytes of K and of q
+          const u32x4 kq = *reinterpret_cast<const u32x4*>(k + j * p.ks[1] + d);
+          const u32x4 qq = *reinterpret_cast<const u32x4*>(qr + d);
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            const uint32_t a = kq[i], b = qq[i];
+            if (sizeof(T) == 2) {
+              x = fmaf(bf16_lo(a), bf16_lo(b), x);
+              x = fmaf(bf16_hi(a), bf16_hi(b), x);
+            } else {
+              x = fmaf(__uint_as_float(a), __uint_as_float(b), x);
+            }
+          }
+        }
         x *= p.c;
         x = x != x ? INFINITY : x;  // a NaN logit: NaN below (inf - inf)
       }
@@ -120,18 +135,30 @@ __device__ __forceinline__ void win_redo_row(const WindowParams& p, const WinTil
 #pragma unroll
       for (int i = 0; i < DPC; ++i) acc[i] *= alpha;
       uint64_t todo = __ballot(seen);
-      while (todo) {
-        const int u = __builtin_ctzll(todo);
-        todo &= todo - 1;
-        const float pu = __shfl(e, u);
-        if (lane * DPC < E) {
+#pragma unroll 1
+      while (todo) {  // AHEAD visible keys at a time, their V rows loaded before any is used
+        float pu[AHEAD], vu[AHEAD][DPC];
 #pragma unroll
-          for (int i = 0; i < DPC; ++i) acc[i] = fmaf(pu, f32(v[(k0 + u) * p.vs[1] + lane * DPC + i]), acc[i]);
+        for (int a = 0; a < AHEAD; ++a) {
+          const int u = todo ? __builtin_ctzll(todo) : -1;
+          todo &= todo - 1;
+          pu[a] = u < 0 ? 0.f : __shfl(e, u);
+#pragma unroll
+          for (int i = 0; i < DPC; ++i)
+            vu[a][i] = u >= 0 && dims ? f32(v[(k0 + u) * p.vs[1] + lane * DPC + i]) : 0.f;
         }
+#pragma unroll
+        for (int a = 0; a < AHEAD; ++a)
+#pragma unroll
+          for (int i = 0; i < DPC; ++i) acc[i] = fmaf(pu[a], vu[a][i], acc[i]);
       }
     }
+    bool lost = true;
+#pragma unroll
+    for (int i = 0; i < DPC; ++i) lost &= acc[i] != acc[i];
+    if (!__any(dims && !lost)) break;
   }
-  if (lane * DPC < E) {
+  if (dims) {
 #pragma unroll
     for (int i = 0; i < DPC; ++i) store(m, l, lane * DPC + i, acc[i]);
   }

@@ -358,3 +358,6 @@ def test_workspace_queries():
     assert lib.ca_flash_window_workspace_bytes(1, 4, 8192, 8, 64, 1, 1, -1, -1, 0) \
         == lib.ca_flash_workspace_bytes(1, 4, 8192, 8, 64, 1) > 0
     assert lib.ca_flash_window_workspace_bytes(1, 512, 8192, 8, 64, 1, 1, 100, 0, 0) == 0
+    # splits are at most the 64 that the combine merges
+    for dtype in (0, 1):
+        assert lib.ca_flash_window_workspace_bytes(1, 1, 1 << 20, 1, 64, dtype, 1, 1 << 19, 0, 0) == 64 * 66 * 4

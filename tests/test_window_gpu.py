@@ -33,8 +33,10 @@ def check(q, k, v, left, right, sinks, causal, scale=None):
 
 
 # (N, L, S, H, E, left, right, sinks, causal); bf16 routes by items = N H ceil(L / 128) and the
-# tiles a block can have: key groups past 8 tiles up to 256 items, splits from 16 tiles up
-# to 64 items, one group otherwise.  fp32: 32-row blocks up to 256 items, else 128.
+# tiles a block can have: up to 256 keys one wave per 32 rows, then key groups past 8 tiles up to
+# 256 items, splits from 16 tiles up to 64 items and from 40 up to 170, one group otherwise.
+# fp32: 128-row blocks from 256 (E = 128: 192) of them, 32-row ones from 256, else 16-row
+# ones, split from 4 tiles of 128 keys where they leave half of the CUs idle.
 SHAPES = [
     (1, 1, 1, 1, 64, 0, 0, 0, True),
     (1, 1, 77, 2, 32, 3, 0, 2, True),
@@ -54,6 +56,10 @@ SHAPES = [
     (1, 40, 3000, 2, 64, 2500, 0, 4, True),     # splits
     (2, 130, 2500, 3, 128, 2100, 3, 65, False),
     (1, 4, 4000, 8, 32, 3000, 0, 1, True),
+    (1, 8, 40000, 1, 64, 39000, 0, 4, True),    # as many as the combine merges
+    (1, 1, 20000, 2, 128, 19000, 0, 1, True),
+    (1, 700, 6000, 12, 64, 4500, 0, 4, True),   # 72 and 108 items
+    (1, 600, 6000, 22, 32, 4500, 100, 0, False),
     (3, 700, 700, 50, 32, 90, 0, 4, True),      # more items than 256
     (2, 500, 500, 40, 64, 450, 0, 130, True),
     (1, 1100, 1100, 33, 128, 129, 0, 16, True),
@@ -135,6 +141,24 @@ def test_unseen_values_stay_out(cuda, dtype, shape, bad):
         assert np.all(np.isfinite(got[~touched])) and np.all(err[~touched] <= clean.bound(NAME[dtype], True)[~touched])
         # rows that see it: not finite where the formula is not
         assert np.array_equal(np.isnan(got[touched]), np.isnan(ref.out[touched]))
+
+
+@pytest.mark.parametrize("dtype", DTYPES, ids=NAME.get)
+def test_nan_queries_stay_in_their_rows(cuda, dtype):
+    for N, L, S, H, E, left in ((1, 200, 100, 2, 64, 60), (1, 700, 700, 2, 128, 600), (1, 40, 3000, 2, 64, 2500)):
+        q, k, v = inputs(N, L, S, H, E, dtype, seed=13)
+        q[0, 3::7, 1, 2] = float("nan")
+        check(q, k, v, left, 0, 4, True)
+
+
+@pytest.mark.parametrize("dtype", DTYPES, ids=NAME.get)
+def test_inputs_of_nothing_but_nans(cuda, dtype):
+    """NaN wherever a row sees a key, soon; zeros elsewhere."""
+    for N, L, S, H, E, left in ((1, 200, 100, 2, 64, 60), (1, 3000, 3000, 4, 128, 2000), (1, 40, 9000, 2, 64, 8000)):
+        q, k, v = (torch.full_like(x, float("nan")) for x in inputs(N, L, S, H, E, dtype))
+        out = C.flash_attn_window_func(q, k, v, window_size=(left, 0), sink_tokens=4)
+        some = torch.arange(L, device=cuda) + S - L >= 0
+        assert bool(out[:, some].isnan().all()) and bool((out[:, ~some] == 0).all())
 
 
 @pytest.mark.parametrize("dtype", DTYPES, ids=NAME.get)
