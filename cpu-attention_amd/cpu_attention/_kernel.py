@@ -106,7 +106,7 @@ class FlashWindowArgs(ctypes.Structure):
 class DecodeWindowArgs(ctypes.Structure):
     """``ca_decode_window_args`` (include/cpu_attention_hip.h)."""
     _fields_ = [("decode", DecodeArgs), ("k_scale", ctypes.c_void_p), ("v_scale", ctypes.c_void_p),
-                ("left", ctypes.c_int64), ("sinks", ctypes.c_int64)]
+                ("left", ctypes.c_int64), ("sinks", ctypes.c_int64), ("longest", ctypes.c_void_p)]
 
 
 class StoreFp8Args(ctypes.Structure):
@@ -133,8 +133,9 @@ _HOST_CHECKS = [os.environ.get("CPU_ATTENTION_HOST_CHECKS", "1") != "0"]
 
 def set_host_checks(enabled):
     """Check slots and lengths against the cache on the host (the reference's
-    ValueErrors; a device sync per call when they live on the GPU). Returns the
-    previous setting."""
+    ValueErrors; a device sync per call when they live on the GPU, or for the window
+    and 8-bit decodes a wait until the call's kernel starts). Returns the previous
+    setting."""
     old = _HOST_CHECKS[0]
     _HOST_CHECKS[0] = bool(enabled)
     if _MODULE is not None and isinstance(_MODULE, NativeModule):

@@ -415,6 +415,7 @@ extern "C" int ca_decode_window(const ca_decode_window_args* wa, void* stream) {
     return CA_DECLINED;
   if (a->num_seqs < 0 || a->num_heads <= 0 || a->num_blocks < 0 || a->page_table_width < 0) return CA_DECLINED;
   if ((wa->k_scale == nullptr) != (wa->v_scale == nullptr) || a->slots) return CA_DECLINED;
+  if ((uintptr_t)wa->longest % 8) return CA_DECLINED;
   if ((a->k_new == nullptr) != (a->v_new == nullptr) || a->new_tokens < 0 || a->new_tokens > (1 << 30)) return CA_DECLINED;
   if (a->num_seqs == 0) return CA_OK;
   // An empty page table or cache is never read: its pointer may be null.
@@ -431,6 +432,7 @@ extern "C" int ca_decode_window(const ca_decode_window_args* wa, void* stream) {
   WinDecodeParams p{};
   p.left = win_left(wa->left, cap);
   p.sinks = wa->sinks < cap ? wa->sinks : cap;
+  p.longest = wa->longest;
   const bool fold = a->k_new && per_seq == 1 && win_decode_folds(rows, a->page_size, f8);
   const int64_t tiles = win_decode_tiles(a->page_table_width, a->page_size, p.left, p.sinks) + (fold && f8 ? 1 : 0);
   if (tiles > 0x7fffffff) return CA_DECLINED;
@@ -440,6 +442,11 @@ extern "C" int ca_decode_window(const ca_decode_window_args* wa, void* stream) {
                       a->workspace_bytes < win_decode_ws_bytes(p.slots, a->head_dim)))
     return CA_DECLINED;
   hipStream_t st = static_cast<hipStream_t>(stream);
+  if (p.longest) {  // a replayed graph would tell a host that no longer listens
+    if (a->k_new && !fold) return CA_DECLINED;
+    hipStreamCaptureStatus capture = hipStreamCaptureStatusNone;
+    if (hipStreamIsCapturing(st, &capture) != hipSuccess || capture != hipStreamCaptureStatusNone) return CA_DECLINED;
+  }
   // One new token per sequence is stored by the decode itself in small calls, others go in
   // first, by a kernel of their own.
   if (fold) {

@@ -67,6 +67,8 @@ struct WinDecodeParams : DecodeParams {
   int64_t new_stride;     // elements from one sequence's new token to the next's
   float* k_scale_store;   // the scales, writable
   float* v_scale_store;
+  int64_t* longest;       // receives max(lens, 0) as the decode starts, and nothing is
+                          // appended if that is past the table (nullptr: nobody asks)
 };
 
 // A cache of e4m3 codes and the tokens that go into it.

@@ -68,6 +68,15 @@ __device__ __forceinline__ Span span_of(const WinDecodeParams& p, int64_t seq) {
   return x;
 }
 
+// The largest length, 0 if that is negative.
+__device__ __forceinline__ int64_t longest_of(const WinDecodeParams& p) {
+  int32_t longest = 0;
+  for (int64_t i = threadIdx.x & 63; i < p.nseqs; i += kWave) longest = max(longest, p.lens[i]);
+#pragma unroll
+  for (int d = kWave / 2; d; d /= 2) longest = max(longest, __shfl_xor(longest, d));
+  return longest;
+}
+
 // The low n bits (n <= 0: none, n >= 16: all of a unit).
 __device__ __forceinline__ uint32_t low_bits(int64_t n) {
   return n <= 0 ? 0u : (n >= kUnit ? 0xffffu : (1u << (int)n) - 1u);
@@ -124,7 +133,9 @@ __device__ __forceinline__ void win_tile(const WinDecodeParams& p, const Span& s
   const bool final = tile == sp.tiles - 1;
   const int64_t iu = (final ? sp.last : tile * NU) + lane;
   // The new token: at position lens[seq], the row's newest unless that lies past the table.
-  const bool fresh = APPEND && final && sp.len > 0 && p.lens[seq] == sp.len - 1;
+  // A host that has such lengths refused (longest) wants no sequence's token stored then.
+  bool fresh = APPEND && final && sp.len > 0 && p.lens[seq] == sp.len - 1;
+  if (APPEND && fresh && p.longest && p.nseqs > 1) fresh = longest_of(p) < p.pt_width * p.page;
   if constexpr (APPEND && F8) {
     if (fresh) {
       const int64_t pi = page_of(sp.len - 1, p.page), at = sp.len - 1 - pi * p.page;
@@ -376,6 +387,11 @@ __global__ __launch_bounds__(64 * kDecWaves) void win_decode_kernel(WinDecodePar
   const int64_t row = blockIdx.x;
   const int64_t s = (uint32_t)row / (uint32_t)p.heads, h = row - s * p.heads;
   const int64_t tile = (int64_t)blockIdx.y * kDecWaves + wv;
+  // For a host that polls it while the decode runs; nothing else has to be visible with it.
+  if (p.longest && (blockIdx.x | blockIdx.y) == 0 && wv == 0) {
+    const int64_t longest = longest_of(p);
+    if ((threadIdx.x & 63) == 0) __hip_atomic_store(p.longest, longest, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_SYSTEM);
+  }
   const Span sp = span_of<APPEND && F8>(p, s);
   // Waves past the row's last tile exit (the barrier below waits for the others only).  A
   // row with no key has one tile of nothing, and is written as exactly 0.

@@ -259,13 +259,22 @@ int ca_flash_window(const ca_flash_window_args* args, void* stream);
  * ca_store_fp8's rule, and sequences of one call must not share the pages they
  * append to.  decode.slots must be NULL.  decode.scale must be positive and finite.
  * decode.workspace: at least ca_decode_window_workspace_bytes(...) bytes (0: none),
- * 16-byte aligned, not initialised; calls that overlap must not share it. */
+ * 16-byte aligned, not initialised; calls that overlap must not share it.
+ *
+ * A length past the page table's capacity is cut off at it.  longest (may be NULL): pinned
+ * host memory, 8-byte aligned, for a host that has such lengths refused without waiting
+ * for lens first.  The call's first block stores the largest of lens there (0 if that is
+ * negative) as it starts, and nothing is appended if a length plus the new token is past
+ * the capacity.  Such a call is declined, with nothing launched, on a stream under capture
+ * and where the new tokens are stored ahead of the decode (more than one per sequence, many
+ * rows, long pages of the 8-bit cache). */
 typedef struct ca_decode_window_args {
   ca_decode_args decode;
   float* k_scale;
   float* v_scale;
   int64_t left;
   int64_t sinks;
+  int64_t* longest;
 } ca_decode_window_args;
 
 int64_t ca_decode_window_workspace_bytes(int64_t num_seqs, int64_t num_heads, int64_t head_dim,

@@ -2,6 +2,8 @@
 oracle, within bounds derived from the arithmetic.  Everything that a row does not see is
 NaN (cache positions, pages, scales) or out of range (page-table entries)."""
 
+import ctypes
+
 import numpy as np
 import pytest
 import torch
@@ -305,3 +307,84 @@ def test_empty_batch_and_empty_cache(cuda):
         assert call(p, fp8, q=p.q[:0], lens=p.lens_t[:0], table=p.table[:0], window_size=(3, 0)).shape == (0, 1, 2, 64)
         zero = torch.zeros(1, dtype=torch.int32, device=cuda)
         assert bool((call(p, fp8, lens=zero, table=p.table[:, :0], window_size=(3, 0)) == 0).all())
+
+
+@pytest.mark.parametrize("dtype,fp8", KINDS, ids=IDS)
+@pytest.mark.parametrize("seqs,heads,n", [(3, 2, 0), (3, 2, 1), (1, 1, 1), (100, 2, 1), (3, 2, 5), (70, 16, 1)])
+def test_a_length_past_the_table_stores_nothing(cuda, dtype, fp8, seqs, heads, n):
+    """With host checks on, whichever sequence's length it is, whether the decode stores the
+    token itself or a kernel before it does."""
+    p = Paged([(20 + 7 * i) % 60 for i in range(seqs)], heads, 32, 16, dtype, 14, cuda, fp8=fp8, spare=8)
+    room = p.table.shape[1] * 16
+    kv = {}
+    if n:
+        k, v = torch.randn(2, seqs, n, heads, 32, device=cuda).to(dtype) * 100
+        kv = {"k": k, "v": v}
+    state = [p.kc, p.vc] + ([p.kscale, p.vscale] if fp8 else [])
+    before = [x.clone() for x in state]
+    for i in sorted({0, seqs // 2, seqs - 1}):
+        lens = p.lens_t.clone()
+        lens[i] = room + 1 - n
+        for where in (lens, lens.cpu()):
+            with pytest.raises(ValueError, match="exceed the page table's capacity"):
+                call(p, fp8, lens=where, window_size=(30, 0), sink_tokens=2, **kv)
+        torch.cuda.synchronize()
+        assert all(same_bytes(x, y) for x, y in zip(state, before))
+    out = call(p, fp8, window_size=(30, 0), sink_tokens=2)
+    close(out, reference(p, 30, 2), dtype)
+    with torch.cuda.stream(torch.cuda.Stream()):
+        torch.cuda.current_stream().wait_stream(torch.cuda.default_stream())
+        assert same_bytes(call(p, fp8, window_size=(30, 0), sink_tokens=2), out)
+
+
+@pytest.mark.parametrize("fp8", [False, True], ids=["bf16", "fp8"])
+def test_longest_at_the_c_entry(cuda, fp8):
+    p = Paged([100, 300, 16], 2, 64, 16, BF16, 15, cuda, fp8=fp8, spare=4)
+    lib = K.load_library()
+    out = torch.empty_like(p.q)
+    slot = torch.full((2,), -1, dtype=torch.int64).pin_memory()
+    a = K.DecodeWindowArgs()
+    d = a.decode
+    d.q, d.q_stride, d.out, d.lens = p.q.data_ptr(), p.q.stride(0), out.data_ptr(), p.lens_t.data_ptr()
+    d.k_cache, d.v_cache = p.kc.data_ptr(), p.vc.data_ptr()
+    d.page_table, d.page_table_width = p.table.data_ptr(), p.table.shape[1]
+    d.scale, d.num_seqs, d.num_heads, d.head_dim = 64 ** -0.5, 3, 2, 64
+    d.page_size, d.num_blocks, d.dtype = 16, p.blocks, K.DTYPES[BF16]
+    a.left, a.sinks = 200, 4
+    if fp8:
+        a.k_scale, a.v_scale = p.kscale.data_ptr(), p.vscale.data_ptr()
+    need = lib.ca_decode_window_workspace_bytes(3, 2, 64, 16, d.page_table_width, a.left, a.sinks)
+    ws = torch.empty(max(need, 16), dtype=torch.uint8, device=cuda)
+    d.workspace, d.workspace_bytes = ws.data_ptr(), need
+    run = lambda: lib.ca_decode_window(ctypes.byref(a), torch.cuda.current_stream().cuda_stream)
+    want = call(p, fp8, window_size=(200, 0), sink_tokens=4)
+    for lens, longest in ((p.lens, 300), ([-4, -1, -9], 0)):
+        p.lens_t.copy_(torch.tensor(lens, dtype=torch.int32))
+        slot.fill_(-1)
+        a.longest = slot.data_ptr()
+        assert run() == K.CA_OK
+        torch.cuda.synchronize()
+        assert slot.tolist() == [longest, -1]
+        assert same_bytes(out, want) or longest == 0 and bool((out == 0).all())
+    a.longest = slot.data_ptr() + 4
+    assert run() == K.CA_DECLINED
+    p.lens_t.copy_(torch.tensor(p.lens, dtype=torch.int32))
+    a.longest = slot.data_ptr()
+    k = torch.zeros(3, 2, 2, 64, dtype=BF16, device=cuda)
+    d.k_new = d.v_new = k.data_ptr()
+    d.kv_stride, d.new_tokens = k.stride(1), 2
+    assert run() == K.CA_DECLINED  # two new tokens each: stored ahead of the decode
+    d.k_new = d.v_new = None
+    d.kv_stride = d.new_tokens = 0
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        declined = run()
+        a.longest = None
+        captured = run()
+    assert (declined, captured) == (K.CA_DECLINED, K.CA_OK)
+    for _ in range(2):
+        out.zero_()
+        graph.replay()
+        torch.cuda.synchronize()
+        assert same_bytes(out, want)
