@@ -608,7 +608,7 @@ class Module:
         page, nblocks = k_cache.shape[2], k_cache.shape[0]
         if _HOST_CHECKS[0] and n and int(slots.max()) >= nblocks * page:
             return None
-        if n == 0 or nblocks == 0:
+        if n == 0 or nblocks == 0 or heads == 0:
             return True
         with torch.cuda.device(dev):
             slots = _index_on(slots, dev)

@@ -352,6 +352,8 @@ def flash_attn_window_func(q, k, v, window_size=(-1, -1), sink_tokens=0, softmax
     rt, flash, _ = _WINDOW_ENTRIES or _window_entries()
     out = flash(rt, q, k, v, softmax_scale, causal, left, right, sinks)
     if out is None:
+        if k.dim() == 4 and k.shape[2] == 0:
+            raise ValueError("cpu_attention: q/k/v need at least one head")
         q, k, v = _check_flash(q, k, v)
         out = flash(rt, q, k, v, softmax_scale, bool(causal), left, right, sinks)
         if out is None:  # strides past the kernels' 32-bit tile offsets

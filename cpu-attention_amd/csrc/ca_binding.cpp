@@ -132,7 +132,7 @@ class Longest {
   }
   int64_t* slot() const { return slot_.data_ptr<int64_t>(); }
   int64_t wait() const {
-    for (int spins = 0;; ++spins) {
+    for (uint32_t spins = 0;; ++spins) {
       const int64_t v = __atomic_load_n(slot(), __ATOMIC_RELAXED);
       if (v >= 0) return v;
       // The end of the stream's work (or an error of it, which raises) is the end of the wait.
@@ -691,7 +691,7 @@ static PyObject* b_store_fp8(PyObject*, PyObject* const* args, Py_ssize_t nargs)
   if (kc.numel() && kc.data_ptr() == vc.data_ptr()) Py_RETURN_NONE;
   const int64_t page = kc.size(2), nblocks = kc.size(0);
   if (g_host_checks && n && max_of(T(slo)) >= nblocks * page) Py_RETURN_NONE;
-  if (n == 0 || nblocks == 0) Py_RETURN_TRUE;
+  if (n == 0 || nblocks == 0 || heads == 0) Py_RETURN_TRUE;
   const c10::DeviceGuard guard(dev);
   void* stream;
   if (!stream_of(dev, &stream)) return nullptr;

@@ -217,3 +217,12 @@ def test_bindings_agree(cuda):
         assert K.module().store_fp8(K.runtime(), key, value, *a.gpu, slots) is True
         assert K.ctypes_module().store_fp8(K.runtime(), key, value, *b.gpu, slots) is True
         assert all(same_bytes(x, y) for x, y in zip(a.gpu, b.gpu))
+
+
+def test_no_heads_and_no_pages(cuda):
+    for heads, blocks in ((0, 4), (2, 0)):
+        kc, vc = (torch.zeros(blocks, heads, 16, 64, device=cuda).to(torch.float8_e4m3fn) for _ in range(2))
+        ks, vs = (torch.zeros(blocks, heads, device=cuda) for _ in range(2))
+        key = torch.ones(3, heads, 64, device=cuda)
+        C.reshape_and_cache_fp8(key, key, kc, vc, ks, vs, torch.full((3,), -1, device=cuda))
+        assert K.ctypes_module().store_fp8(K.runtime(), key, key, kc, vc, ks, vs, torch.full((3,), -1, device=cuda)) is True

@@ -361,3 +361,11 @@ def test_workspace_queries():
     # splits are at most the 64 that the combine merges
     for dtype in (0, 1):
         assert lib.ca_flash_window_workspace_bytes(1, 1, 1 << 20, 1, 64, dtype, 1, 1 << 19, 0, 0) == 64 * 66 * 4
+
+
+def test_no_heads():
+    q = torch.zeros(1, 4, 0, 64)
+    with pytest.raises(ValueError, match="at least one head"):
+        C.flash_attn_window_func(q, q, q, window_size=(2, 0))
+    with pytest.raises(ValueError, match="at least one head"):
+        C.flash_attn_window_func(torch.zeros(1, 4, 2, 64), q, q, window_size=(2, 0))
