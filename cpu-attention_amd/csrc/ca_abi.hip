@@ -396,7 +396,19 @@ extern "C" int ca_flash_window(const ca_flash_window_args* wa, void* stream) {
 
 static int64_t win_left(int64_t left, int64_t cap) { return left < 0 || left >= cap ? -1 : left; }
 
-static int64_t win_decode_ws_bytes(int64_t slots, int64_t head_dim) { return decode_acc_bytes(slots, head_dim) + slots * 8; }
+// Window and 8-bit decodes whose split rows are merged by their last block inside the
+// kernel: ca_decode's limits from 64 rows on, and 3 blocks a row for fewer (their second
+// launch is a larger part of the call).  Second launch / in-kernel, us per call with a
+// one-token append: 32 rows E=128, 3 blocks 12.2 / 11.5, 4 blocks 12.8 / 13.5, 8-bit 11.0 /
+// 11.8; 8 rows E=64, 2 blocks 10.3 / 7.9; 128 rows 3 blocks 17.8 / 17.6, fp32 E=64 17.6 /
+// 17.0, 8-bit 14.5 / 13.9; 512 rows E=64 36.8 / 35.5.
+static bool win_decode_merges(int64_t rows, int64_t slots) {
+  return slots > 0 && rows <= kMergeMaxRows && slots <= rows * (rows < kMergeMinRows ? 3 : kMergeMaxBlocks);
+}
+
+static int64_t win_decode_ws_bytes(int64_t rows, int64_t slots, int64_t head_dim) {
+  return decode_acc_bytes(slots, head_dim) + slots * 8 + (win_decode_merges(rows, slots) ? rows * 8 : 0);
+}
 
 extern "C" int64_t ca_decode_window_workspace_bytes(int64_t num_seqs, int64_t num_heads, int64_t head_dim,
                                                     int64_t page_size, int64_t page_table_width, int64_t left,
@@ -405,7 +417,8 @@ extern "C" int64_t ca_decode_window_workspace_bytes(int64_t num_seqs, int64_t nu
   const int64_t cap = page_table_width * page_size;
   const int64_t tiles = win_decode_tiles(page_table_width, page_size, win_left(left, cap), sinks < cap ? sinks : cap);
   // One tile more: an 8-bit cache's last page, if the call appends to it.
-  return win_decode_ws_bytes(win_decode_slots(num_seqs * num_heads, tiles + 1), head_dim);
+  const int64_t rows = num_seqs * num_heads;
+  return win_decode_ws_bytes(rows, win_decode_slots(rows, tiles + 1), head_dim);
 }
 
 extern "C" int ca_decode_window(const ca_decode_window_args* wa, void* stream) {
@@ -439,7 +452,7 @@ extern "C" int ca_decode_window(const ca_decode_window_args* wa, void* stream) {
   p.tiles = (int)tiles;
   p.slots = win_decode_slots(rows, p.tiles);
   if (p.slots > 0 && (!a->workspace || !aligned16(a->workspace) ||
-                      a->workspace_bytes < win_decode_ws_bytes(p.slots, a->head_dim)))
+                      a->workspace_bytes < win_decode_ws_bytes(rows, p.slots, a->head_dim)))
     return CA_DECLINED;
   hipStream_t st = static_cast<hipStream_t>(stream);
   if (p.longest) {  // a replayed graph would tell a host that no longer listens
@@ -512,6 +525,10 @@ extern "C" int ca_decode_window(const ca_decode_window_args* wa, void* stream) {
   p.c = a->scale * kLog2e;
   p.part_acc = static_cast<float*>(a->workspace);
   p.part_ml = reinterpret_cast<float*>(static_cast<char*>(a->workspace) + decode_acc_bytes(p.slots, a->head_dim));
+  if (win_decode_merges(rows, p.slots)) {
+    p.counters = reinterpret_cast<uint64_t*>(p.part_ml + 2 * p.slots);
+    p.tag = next_merge_tag();
+  }
   p.out = a->out;
   p.k_scale = wa->k_scale;
   p.v_scale = wa->v_scale;

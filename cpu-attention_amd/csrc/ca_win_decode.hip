@@ -11,7 +11,8 @@
 // Only what the row sees is walked: the 16-key units that hold a sink or a window key,
 // numbered without the gap between them (Span).  The grid covers the most units that a
 // row of the call's window can have, not the page table's capacity.  One wave takes a
-// tile of TK keys (TK / 16 units), a block 8 tiles; a unit's visible keys are 16 bits of
+// tile of TK keys (TK / 16 units), a block 8 tiles, merged in LDS; a row of more blocks is
+// merged by its last one, or (many rows or blocks) by a second kernel.  A unit's visible keys are 16 bits of
 // a mask, which decides what is read: a masked key's V row is never loaded, and its
 // logit is -inf whatever its K holds.
 //
@@ -377,6 +378,35 @@ __device__ __forceinline__ void win_tile(const WinDecodeParams& p, const Span& s
   }
 }
 
+// In-kernel merge of a row's nrow blocks: this block's partial (mx, l, acc) goes to `slot`
+// and the row's last block writes the row.  The partial is written with agent-scope atomic
+// stores, which the hardware makes visible device-wide (they write through the XCD's L2) by
+// the time the wave's store counter reaches zero; only then does the block count itself in
+// on the row's counter.  The block that completes the count has seen every other block's
+// count, hence every other partial, and reads them with agent-scope atomic loads: no L2
+// write-back or invalidation, which agent-scope fences would do for the whole L2.
+template <int E, bool BF, int DPC>
+__device__ __forceinline__ void merge_in_last_block(const DecodeParams& p, int64_t row, int64_t slot, int nrow, float mx,
+                                                    float l, const float (&acc)[DPC], int lane) {
+  if (lane * DPC < E) {
+#pragma unroll
+    for (int i = 0; i < DPC; ++i)
+      __hip_atomic_store(p.part_acc + slot * E + lane * DPC + i, acc[i], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+  }
+  if (lane == 0) {
+    __hip_atomic_store(p.part_ml + 2 * slot, mx, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    __hip_atomic_store(p.part_ml + 2 * slot + 1, l, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+  }
+  asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+  int arrived = 0;
+  if (lane == 0) arrived = merge_count_in(p.counters + row, p.tag);
+  arrived = __builtin_amdgcn_readfirstlane(arrived);
+  if (arrived != nrow) return;
+  asm volatile("" ::: "memory");
+  if (lane == 0) __hip_atomic_store(p.counters + row, (uint64_t)0, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+  merge_partials<E, BF, true>(p, row, nrow, lane);
+}
+
 template <int E, bool BF, bool F8, bool APPEND, int TK>
 __global__ __launch_bounds__(64 * kDecWaves) void win_decode_kernel(WinDecodeParams p) {
   __shared__ __attribute__((aligned(16))) float p_lds[kDecWaves][TK];
@@ -411,6 +441,10 @@ __global__ __launch_bounds__(64 * kDecWaves) void win_decode_kernel(WinDecodePar
     return;
   }
   const int64_t slot = row * cdiv(p.tiles, kDecWaves) + blockIdx.y;
+  if (p.counters) {
+    merge_in_last_block<E, BF>(p, row, slot, (int)cdiv(sp.tiles, kDecWaves), mx, l, acc, lane);
+    return;
+  }
   if (lane * DPC < E) {
 #pragma unroll
     for (int i = 0; i < DPC; ++i) p.part_acc[slot * E + lane * DPC + i] = acc[i];
@@ -421,7 +455,8 @@ __global__ __launch_bounds__(64 * kDecWaves) void win_decode_kernel(WinDecodePar
   }
 }
 
-// One wave per row of more than one block: merges the blocks' partials.
+// One wave per row of more than one block, where the rows' last blocks do not: merges the
+// blocks' partials.
 template <int E, bool BF, bool FOLD>
 __global__ __launch_bounds__(256) void win_decode_combine_kernel(WinDecodeParams p) {
   const int lane = threadIdx.x & 63;
@@ -464,7 +499,7 @@ static int win_decode_launch_t(const WinDecodeParams& p, hipStream_t stream) {
   else
     hipLaunchKernelGGL((win_decode_kernel<E, BF, F8, false, kWinTile>), grid, block, 0, stream, p);
   const int st = ca_launch_status();
-  if (st != CA_OK || gy == 1) return st;
+  if (st != CA_OK || gy == 1 || p.counters) return st;
   const dim3 cg((unsigned)cdiv(rows, 4));
   if (F8 && p.k_new)
     hipLaunchKernelGGL((win_decode_combine_kernel<E, BF, true>), cg, dim3(256), 0, stream, p);

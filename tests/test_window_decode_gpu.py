@@ -388,3 +388,61 @@ def test_longest_at_the_c_entry(cuda, fp8):
         graph.replay()
         torch.cuda.synchronize()
         assert same_bytes(out, want)
+
+
+@pytest.mark.parametrize("dtype,fp8", KINDS, ids=IDS)
+@pytest.mark.parametrize("seqs,heads,left", [(3, 2, 1000), (3, 2, 1300), (3, 2, 1700), (8, 8, 1700), (8, 8, 2200),
+                                             (32, 16, 900), (34, 16, 900)])
+def test_rows_of_several_blocks(cuda, dtype, fp8, seqs, heads, left):
+    """2 to 5 blocks of 512 keys a row, rows of one block among them: merged by the row's last
+    block or by a second kernel, whatever the workspace holds, replayed in a graph too."""
+    g = torch.Generator().manual_seed(16)
+    lens = [int(x) for x in torch.randint(1, 2600, (seqs,), generator=g)]
+    lens[0], lens[-1] = 2599, 7
+    p = Paged(lens, heads, 32, 64, dtype, 17, cuda, fp8=fp8)
+    lib = K.load_library()
+    out = torch.empty_like(p.q)
+    a = K.DecodeWindowArgs()
+    d = a.decode
+    d.q, d.q_stride, d.out, d.lens = p.q.data_ptr(), p.q.stride(0), out.data_ptr(), p.lens_t.data_ptr()
+    d.k_cache, d.v_cache = p.kc.data_ptr(), p.vc.data_ptr()
+    d.page_table, d.page_table_width = p.table.data_ptr(), p.table.shape[1]
+    d.scale, d.num_seqs, d.num_heads, d.head_dim = 32 ** -0.5, seqs, heads, 32
+    d.page_size, d.num_blocks, d.dtype = 64, p.blocks, K.DTYPES[dtype]
+    a.left, a.sinks = left, 3
+    if fp8:
+        a.k_scale, a.v_scale = p.kscale.data_ptr(), p.vscale.data_ptr()
+    need = lib.ca_decode_window_workspace_bytes(seqs, heads, 32, 64, d.page_table_width, left, 3)
+    assert need > 0
+    ws = torch.zeros(need, dtype=torch.uint8, device=cuda)
+    d.workspace, d.workspace_bytes = ws.data_ptr(), need
+
+    def run():
+        assert lib.ca_decode_window(ctypes.byref(a), torch.cuda.current_stream().cuda_stream) == K.CA_OK
+
+    run()
+    first = out.clone()
+    some = sorted({0, seqs // 2, seqs - 1})
+    close(first[some], R.decode(values(p.q)[some, 0], [p.ks[i] for i in some], [p.vs[i] for i in some], 32 ** -0.5, left, 3),
+          dtype)
+    for i in range(12):
+        if i % 3 == 0:
+            ws.fill_(0 if i % 2 else 255)
+        elif i % 3 == 1:
+            ws.random_(0, 256)
+        out.zero_()
+        run()
+        assert same_bytes(out, first)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        run()
+    for i in range(4):
+        out.zero_()
+        if i == 2:
+            ws.random_(0, 256)
+        graph.replay()
+        torch.cuda.synchronize()
+        assert same_bytes(out, first)
+        run()
+        assert same_bytes(out, first)
