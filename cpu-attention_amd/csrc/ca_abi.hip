@@ -397,13 +397,14 @@ extern "C" int ca_flash_window(const ca_flash_window_args* wa, void* stream) {
 static int64_t win_left(int64_t left, int64_t cap) { return left < 0 || left >= cap ? -1 : left; }
 
 // Window and 8-bit decodes whose split rows are merged by their last block inside the
-// kernel: ca_decode's limits from 64 rows on, and 3 blocks a row for fewer (their second
-// launch is a larger part of the call).  Second launch / in-kernel, us per call with a
-// one-token append: 32 rows E=128, 3 blocks 12.2 / 11.5, 4 blocks 12.8 / 13.5, 8-bit 11.0 /
-// 11.8; 8 rows E=64, 2 blocks 10.3 / 7.9; 128 rows 3 blocks 17.8 / 17.6, fp32 E=64 17.6 /
-// 17.0, 8-bit 14.5 / 13.9; 512 rows E=64 36.8 / 35.5.
+// kernel: up to 512 rows of 4 blocks, or 32 rows of 8.  Second launch / in-kernel, us per
+// call with a one-token append, bf16 unless noted: 8 rows E=64, 2 blocks 10.3 / 7.9, 8 blocks 9.3 /
+// 8.4, 16 blocks 10.9 / 11.5, 63 blocks 21.8 / 36; 32 rows E=128, 3 blocks 12.2 / 10.6, 4
+// blocks 12.7 / 11.4 (8-bit 11.1 / 9.8), 8 blocks 16.6 / 16.0, E=64 16 blocks 16.9 / 23; 64 rows
+// 7 blocks E=64 15.8 / 16.8, E=128 24.3 / 23.6; 128 rows E=64 5 blocks 19.4 / 19.8; 512 rows
+// 4 blocks 78.2 / 78.2, 5 blocks E=64 55.2 / 56.9; 1024 rows E=64, 3 blocks 63.3 / 64.2.
 static bool win_decode_merges(int64_t rows, int64_t slots) {
-  return slots > 0 && rows <= kMergeMaxRows && slots <= rows * (rows < kMergeMinRows ? 3 : kMergeMaxBlocks);
+  return slots > 0 && rows <= kMergeMaxRows && slots <= rows * (rows <= 32 ? 8 : kMergeMaxBlocks);
 }
 
 static int64_t win_decode_ws_bytes(int64_t rows, int64_t slots, int64_t head_dim) {

@@ -105,20 +105,4 @@ __device__ __forceinline__ void merge_partials(const DecodeParams& p, int64_t ro
   if (dims) store_out<DPC, BF>(p.out, row * E + lane * DPC, acc, l > 0.f ? 1.f / l : 0.f);
 }
 
-// Counts one more block of a row in: the counter word holds the call's tag (high
-// 32 bits) and the blocks counted so far (low 32).  A word with another tag (a
-// fresh workspace's contents, or 0, which the row's last block leaves behind and
-// no call uses as its tag) counts as none.  Returns the count including this
-// block.  Each failed compare-and-swap means another block's succeeded, so the
-// loop ends after at most one try per block of the row.
-__device__ __forceinline__ int merge_count_in(uint64_t* ctr, uint32_t tag) {
-  uint64_t cur = __hip_atomic_load(ctr, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-  for (;;) {
-    const uint64_t want = (uint32_t)(cur >> 32) == tag ? cur + 1 : ((uint64_t)tag << 32) | 1u;
-    if (__hip_atomic_compare_exchange_strong(ctr, &cur, want, __ATOMIC_RELAXED, __ATOMIC_RELAXED,
-                                             __HIP_MEMORY_SCOPE_AGENT))
-      return (int)(uint32_t)want;
-  }
-}
-
 }  // namespace ca

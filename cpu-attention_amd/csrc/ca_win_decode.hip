@@ -12,9 +12,9 @@
 // numbered without the gap between them (Span).  The grid covers the most units that a
 // row of the call's window can have, not the page table's capacity.  One wave takes a
 // tile of TK keys (TK / 16 units), a block 8 tiles, merged in LDS; a row of more blocks is
-// merged by its last one, or (many rows or blocks) by a second kernel.  A unit's visible keys are 16 bits of
-// a mask, which decides what is read: a masked key's V row is never loaded, and its
-// logit is -inf whatever its K holds.
+// merged by its last one, or (many rows or blocks) by a second kernel.  A unit's visible
+// keys are 16 bits of a mask, which decides what is read: a masked key's V row is never
+// loaded, and its logit is -inf whatever its K holds.
 //
 // Bound: reading the visible keys once (HBM).
 #include "ca_device.h"
@@ -379,15 +379,28 @@ __device__ __forceinline__ void win_tile(const WinDecodeParams& p, const Span& s
 }
 
 // In-kernel merge of a row's nrow blocks: this block's partial (mx, l, acc) goes to `slot`
-// and the row's last block writes the row.  The partial is written with agent-scope atomic
-// stores, which the hardware makes visible device-wide (they write through the XCD's L2) by
-// the time the wave's store counter reaches zero; only then does the block count itself in
-// on the row's counter.  The block that completes the count has seen every other block's
-// count, hence every other partial, and reads them with agent-scope atomic loads: no L2
-// write-back or invalidation, which agent-scope fences would do for the whole L2.
+// and the row's last block writes the row.
+//
+// The row's counter word holds the call's tag (high 32 bits) and the blocks counted so far
+// (low 32).  A word with another tag (a fresh workspace's contents, or 0, which the last
+// block leaves behind and no call's tag is) is first made the tag with none counted:
+// `seen` is the word as this block read it, and where that swap fails another block's has
+// succeeded.  Then every block adds itself once, so nothing is tried again however many
+// finish together.
+//
+// The partial is written with agent-scope atomic stores, which the hardware makes visible
+// device-wide (they write through the XCD's L2) by the time the wave's store counter
+// reaches zero; only then does the block count itself in.  The block that completes the
+// count has seen every other block's count, hence every other partial, and reads them with
+// agent-scope atomic loads: no L2 write-back or invalidation, which agent-scope fences
+// would do for the whole L2.
 template <int E, bool BF, int DPC>
-__device__ __forceinline__ void merge_in_last_block(const DecodeParams& p, int64_t row, int64_t slot, int nrow, float mx,
-                                                    float l, const float (&acc)[DPC], int lane) {
+__device__ __forceinline__ void merge_in_last_block(const DecodeParams& p, int64_t row, int64_t slot, int nrow, uint64_t seen,
+                                                    float mx, float l, const float (&acc)[DPC], int lane) {
+  uint64_t* ctr = p.counters + row;
+  if (lane == 0 && (uint32_t)(seen >> 32) != p.tag)
+    __hip_atomic_compare_exchange_strong(ctr, &seen, (uint64_t)p.tag << 32, __ATOMIC_RELAXED, __ATOMIC_RELAXED,
+                                         __HIP_MEMORY_SCOPE_AGENT);
   if (lane * DPC < E) {
 #pragma unroll
     for (int i = 0; i < DPC; ++i)
@@ -399,11 +412,11 @@ __device__ __forceinline__ void merge_in_last_block(const DecodeParams& p, int64
   }
   asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
   int arrived = 0;
-  if (lane == 0) arrived = merge_count_in(p.counters + row, p.tag);
+  if (lane == 0) arrived = (int)(uint32_t)__hip_atomic_fetch_add(ctr, (uint64_t)1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) + 1;
   arrived = __builtin_amdgcn_readfirstlane(arrived);
   if (arrived != nrow) return;
   asm volatile("" ::: "memory");
-  if (lane == 0) __hip_atomic_store(p.counters + row, (uint64_t)0, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+  if (lane == 0) __hip_atomic_store(ctr, (uint64_t)0, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
   merge_partials<E, BF, true>(p, row, nrow, lane);
 }
 
@@ -427,6 +440,8 @@ __global__ __launch_bounds__(64 * kDecWaves) void win_decode_kernel(WinDecodePar
   // row with no key has one tile of nothing, and is written as exactly 0.
   if (tile >= sp.tiles) return;
   win_tile<E, BF, F8, APPEND, TK>(p, sp, s, h, tile, p_lds[wv], part[wv], kl);
+  uint64_t seen = 0;
+  if (p.counters && wv == 0) seen = __hip_atomic_load(p.counters + row, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
   __syncthreads();
   if (wv != 0) return;
   constexpr int DPC = E >= 64 ? E / 64 : 1;
@@ -442,7 +457,7 @@ __global__ __launch_bounds__(64 * kDecWaves) void win_decode_kernel(WinDecodePar
   }
   const int64_t slot = row * cdiv(p.tiles, kDecWaves) + blockIdx.y;
   if (p.counters) {
-    merge_in_last_block<E, BF>(p, row, slot, (int)cdiv(sp.tiles, kDecWaves), mx, l, acc, lane);
+    merge_in_last_block<E, BF>(p, row, slot, (int)cdiv(sp.tiles, kDecWaves), seen, mx, l, acc, lane);
     return;
   }
   if (lane * DPC < E) {

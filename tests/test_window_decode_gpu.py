@@ -391,10 +391,10 @@ def test_longest_at_the_c_entry(cuda, fp8):
 
 
 @pytest.mark.parametrize("dtype,fp8", KINDS, ids=IDS)
-@pytest.mark.parametrize("seqs,heads,left", [(3, 2, 1000), (3, 2, 1300), (3, 2, 1700), (8, 8, 1700), (8, 8, 2200),
+@pytest.mark.parametrize("seqs,heads,left", [(3, 2, 1000), (3, 2, 1300), (3, 2, 1700), (3, 2, 2560), (8, 8, 1700), (8, 8, 2200),
                                              (32, 16, 900), (34, 16, 900)])
 def test_rows_of_several_blocks(cuda, dtype, fp8, seqs, heads, left):
-    """2 to 5 blocks of 512 keys a row, rows of one block among them: merged by the row's last
+    """2 to 6 blocks of 512 keys a row, rows of one block among them: merged by the row's last
     block or by a second kernel, whatever the workspace holds, replayed in a graph too."""
     g = torch.Generator().manual_seed(16)
     lens = [int(x) for x in torch.randint(1, 2600, (seqs,), generator=g)]
