@@ -431,14 +431,20 @@ __global__ __launch_bounds__(64 * kDecWaves) void win_decode_kernel(WinDecodePar
   const int64_t s = (uint32_t)row / (uint32_t)p.heads, h = row - s * p.heads;
   const int64_t tile = (int64_t)blockIdx.y * kDecWaves + wv;
   // For a host that polls it while the decode runs; nothing else has to be visible with it.
-  if (p.longest && (blockIdx.x | blockIdx.y) == 0 && wv == 0) {
-    const int64_t longest = longest_of(p);
-    if ((threadIdx.x & 63) == 0) __hip_atomic_store(p.longest, longest, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_SYSTEM);
-  }
+  // First of all, or behind the row's length, whichever costs less: an append N=1 H=32, window
+  // 1023, 10.6 us against 10.9; without one, 8-bit N=64 H=32 194.5 us against 192.0.
+  auto tell = [&]() __attribute__((always_inline)) {
+    if (p.longest && (blockIdx.x | blockIdx.y) == 0 && wv == 0) {
+      const int64_t longest = longest_of(p);
+      if ((threadIdx.x & 63) == 0) __hip_atomic_store(p.longest, longest, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_SYSTEM);
+    }
+  };
+  if (APPEND) tell();
   const Span sp = span_of<APPEND && F8>(p, s);
   // Waves past the row's last tile exit (the barrier below waits for the others only).  A
   // row with no key has one tile of nothing, and is written as exactly 0.
   if (tile >= sp.tiles) return;
+  if (!APPEND) tell();
   win_tile<E, BF, F8, APPEND, TK>(p, sp, s, h, tile, p_lds[wv], part[wv], kl);
   uint64_t seen = 0;
   if (p.counters && wv == 0) seen = __hip_atomic_load(p.counters + row, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
