@@ -327,8 +327,19 @@ static WindowParams window_params(const FlashParams& f, const WindowSides& w) {
   return p;
 }
 
-static int64_t window_splits(const WindowParams& p, int64_t head_dim, int32_t dtype) {
-  return dtype == CA_BF16 ? flash_window_bf16_splits(p) : flash_window_f32_splits(p, (int)head_dim);
+// What a window call's workspace holds: the partials of `slots` (row, split) pairs, or the
+// words of `blocks` blocks (fp32 on split operands).
+struct WindowSpace {
+  int64_t slots, blocks, bytes;
+};
+static WindowSpace window_space(const WindowParams& p, int64_t head_dim, int32_t dtype) {
+  WindowSpace w{0, dtype == CA_BF16 ? 0 : flash_window_f32_blocks(p, (int)head_dim), 0};
+  if (w.blocks == 0) {
+    const int64_t splits = dtype == CA_BF16 ? flash_window_bf16_splits(p) : flash_window_f32_splits(p, (int)head_dim);
+    if (splits > 1) w.slots = p.batch * p.heads * p.seq_q * splits;
+  }
+  w.bytes = w.slots * (head_dim + 2) * 4 + w.blocks * 4;
+  return w;
 }
 
 extern "C" int64_t ca_flash_window_workspace_bytes(int64_t batch, int64_t seq_q, int64_t seq_k, int64_t num_heads,
@@ -343,8 +354,7 @@ extern "C" int64_t ca_flash_window_workspace_bytes(int64_t batch, int64_t seq_q,
   f.seq_q = seq_q;
   f.seq_k = seq_k;
   f.heads = num_heads;
-  const int64_t splits = window_splits(window_params(f, w), head_dim, dtype);
-  return splits > 1 ? batch * num_heads * seq_q * splits * (head_dim + 2) * 4 : 0;
+  return window_space(window_params(f, w), head_dim, dtype).bytes;
 }
 
 extern "C" int ca_flash_window(const ca_flash_window_args* wa, void* stream) {
@@ -381,17 +391,21 @@ extern "C" int ca_flash_window(const ca_flash_window_args* wa, void* stream) {
   }
   f.c = a->scale * kLog2e;
   WindowParams p = window_params(f, w);
-  const int64_t splits = window_splits(p, a->head_dim, a->dtype);
-  if (splits > 1) {
-    const int64_t slots = a->batch * a->num_heads * a->seq_q * splits;
-    if (!a->workspace || !aligned16(a->workspace) || a->workspace_bytes < slots * (a->head_dim + 2) * 4) return CA_DECLINED;
+  const WindowSpace ws = window_space(p, a->head_dim, a->dtype);
+  if (ws.bytes > 0) {
+    if (!a->workspace || !aligned16(a->workspace) || a->workspace_bytes < ws.bytes) return CA_DECLINED;
     p.part_acc = static_cast<float*>(a->workspace);
-    p.part_ml = p.part_acc + slots * a->head_dim;
+    p.part_ml = p.part_acc + ws.slots * a->head_dim;
     p.workspace_bytes = a->workspace_bytes;
+    if (ws.blocks > 0) p.redo = static_cast<int32_t*>(a->workspace);
   }
   hipStream_t st = static_cast<hipStream_t>(stream);
-  return a->dtype == CA_BF16 ? flash_window_bf16_launch(p, (int)a->head_dim, st)
-                             : flash_window_f32_launch(p, (int)a->head_dim, st);
+  if (a->dtype == CA_BF16) return flash_window_bf16_launch(p, (int)a->head_dim, st);
+  if (ws.blocks > 0) {
+    const int r = flash_window_split_launch(p, (int)a->head_dim, st);
+    if (r != CA_OK) return r;
+  }
+  return flash_window_f32_launch(p, (int)a->head_dim, st);
 }
 
 static int64_t win_left(int64_t left, int64_t cap) { return left < 0 || left >= cap ? -1 : left; }

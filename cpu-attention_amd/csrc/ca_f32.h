@@ -51,6 +51,13 @@
 // us, N=8 L=S=512 H=16 E=64 35.7 -> 37.1, N=1 L=17 S=4096 H=8 E=128 27.6 -> 28.8; N=2
 // L=S=17 H=16 E=128 8.2 -> 8.6).
 //
+// Window calls (P = WindowParams): the tiles are ca_window.h's list, masked by the rows' own
+// limits, and tiles that a wave's rows do not see are left out.  Masked keys take part in
+// the checks like others, so a call with an infinity or NaN among them is redone where they
+// cannot reach a row.  The redo is a launch of its own (ca_win_f32.hip), of the blocks that
+// left a 1 in p.redo: a pass in this kernel costs it registers, the launch 3 us of calls that
+// take 27 or more.
+//
 // Key groups (KG = 2): a second set of 4 waves on the same rows walks every other tile
 // and merges in LDS, as in flash_duo_kernel, for grids that give a CU one block: the
 // waves of one block do not cover each other's softmax and splitting (N=1 L=S=2048 H=32
@@ -173,8 +180,10 @@ inline bool f32_exact(int E, bool causal, int64_t seq_k) {
   return seq_k < kF32TileKeys<128>;
 }
 
-template <int E, int KG, bool SPLIT>
-__global__ __launch_bounds__(256 * KG, 2) void flash_f32_kernel(FlashParams p, int pair) {
+template <int E, int KG, bool SPLIT, class P = FlashParams>
+__global__ __launch_bounds__(256 * KG, 2) void flash_f32_kernel(P p, int pair) {
+  constexpr bool WIN = std::is_same<P, WindowParams>::value;
+  static_assert(!WIN || !SPLIT, "window calls are not split");
   using C = F32Cfg<E>;
   constexpr int BN = C::BN, PL = C::PL, TB = C::TB, CH = C::CH, NS = E / 16, ND = E / 32;
   extern __shared__ __attribute__((aligned(1024))) char f32_smem[];
@@ -212,7 +221,14 @@ __global__ __launch_bounds__(256 * KG, 2) void flash_f32_kernel(FlashParams p, i
     const float* kg = reinterpret_cast<const float*>(p.k) + bw.b * p.ks[0] + bw.h * p.ks[2];
     const float* vg = reinterpret_cast<const float*>(p.v) + bw.b * p.vs[0] + bw.h * p.vs[2];
     const int r0 = (int)bw.q0 + 32 * wv, row = r0 + li;
-    const F32Keys kr = f32_keys(p, bw.q0, SPLIT, sp, splits);
+    WinTiles wt{};
+    F32Keys kr;
+    if constexpr (WIN) {
+      wt = win_tiles(p, (int)bw.q0, kBM, BN);
+      kr = F32Keys{0, 0, wt.n};
+    } else {
+      kr = f32_keys(p, bw.q0, SPLIT, sp, splits);
+    }
     // Group g takes tiles g, g + KG, ...: its round t is tile t KG + g.
     int nkt = (kr.nkt + KG - 1) / KG;
     const int kbeg = (int)kr.kbeg;
@@ -223,8 +239,14 @@ __global__ __launch_bounds__(256 * KG, 2) void flash_f32_kernel(FlashParams p, i
     u32x4 reg[CH];
     const int koff = f32_tile_offset<E>(tid, 0, p.ks[1]), voff = f32_tile_offset<E>(tid, 0, p.vs[1]);
     const int kstep = (int)(RI * p.ks[1] * 4), vstep = (int)(RI * p.vs[1] * 4);
+    // WIN: round t's first key.  A group without a first tile takes the last one's scales.
+    auto win_k0 = [&](int t) __attribute__((always_inline)) {
+      const int i = t * KG + grp;
+      return i < wt.n ? win_key0(wt, i, BN) : (t == 0 ? win_key0(wt, wt.n - 1, BN) : S);
+    };
     auto load_one = [&](const float* g, int64_t stride, int off, int step, int t, u32x4 (&x)[CH]) __attribute__((always_inline)) {
-      const int64_t k0 = kbeg + ((int64_t)t * KG + grp) * BN;
+      int64_t k0 = kbeg + ((int64_t)t * KG + grp) * BN;
+      if constexpr (WIN) k0 = win_k0(t);
       const __amdgpu_buffer_rsrc_t rs = tile_rsrc(g + k0 * stride, f32_tile_bytes<E>(S, k0, stride));
       asm volatile("" : "+v"(off));  // the chunks' offsets are added here, not kept
 #pragma unroll
@@ -233,7 +255,10 @@ __global__ __launch_bounds__(256 * KG, 2) void flash_f32_kernel(FlashParams p, i
     auto load_k = [&](int t, u32x4 (&x)[CH]) __attribute__((always_inline)) { load_one(kg, p.ks[1], koff, kstep, t, x); };
     auto load_v = [&](int t, u32x4 (&x)[CH]) __attribute__((always_inline)) { load_one(vg, p.vs[1], voff, vstep, t, x); };
     // Not ok: the split operands do not serve the query block (Range, above).
-    auto judged = [&](int t) __attribute__((always_inline)) { return S - (kbeg + (t * KG + grp) * BN) >= kF32TileKeys<E>; };
+    auto judged = [&](int t) __attribute__((always_inline)) {
+      if constexpr (WIN) return S - win_k0(t) >= kF32TileKeys<E>;
+      return S - (kbeg + (t * KG + grp) * BN) >= kF32TileKeys<E>;
+    };
     bool ok = nkt == 0 || judged(0);
     float sk = 1.f, sv = 1.f;
     uint32_t* xw = reinterpret_cast<uint32_t*>(f32_smem + C::tiles(KG)) + grp * 4 * C::XW;
@@ -407,8 +432,13 @@ __global__ __launch_bounds__(256 * KG, 2) void flash_f32_kernel(FlashParams p, i
     for (int t = 0; t < nkt; ++t) {
       const uint32_t buf = (t & 1) * TB;
       load_k(t + 1, reg);  // past the last tile: zeros past S, never used
-      const int k0 = kbeg + (t * KG + grp) * BN;
-      const bool mine = k0 < kend_w && (KG == 1 || t * KG + grp < kr.nkt);
+      int k0 = kbeg + (t * KG + grp) * BN;
+      bool mine = k0 < kend_w && (KG == 1 || t * KG + grp < kr.nkt);
+      if constexpr (WIN) {
+        k0 = win_k0(t);
+        mine = r0 < L && t * KG + grp < wt.n && k0 <= r0 + 31 + diag + p.right &&
+               (k0 + BN - 1 >= r0 + diag - p.left || k0 < p.sinks);
+      }
       f32x16 st = f32x16{}, sx = f32x16{};
       if (mine) {
 #pragma unroll
@@ -424,7 +454,19 @@ __global__ __launch_bounds__(256 * KG, 2) void flash_f32_kernel(FlashParams p, i
       if (t + 1 < nkt) store_k(reg, (t & 1) ^ 1);
       load_v(t + 1, reg);
       if (mine) {
-        if (k0 + BN > S || (p.causal && k0 + BN - 1 > r0 + diag)) {
+        if constexpr (WIN) {
+          const int pos = r0 + diag;
+          if (k0 + BN > imin(S, pos + p.right + 1) || (k0 < pos + 31 - p.left && k0 + BN > p.sinks)) {
+            int hi = imin(S - 1, pos + li + p.right) - k0 - 4 * hf, lo = imax(0, pos + li - p.left) - k0 - 4 * hf;
+            int sk = p.sinks - k0 - 4 * hf;
+            asm volatile("" : "+v"(hi), "+v"(lo), "+v"(sk));
+#pragma unroll
+            for (int r = 0; r < 16; ++r) {
+              const int x = 8 * (r >> 2) + (r & 3);
+              st[r] = (x <= hi) & ((x >= lo) | (x < sk)) ? st[r] : -INFINITY;
+            }
+          }
+        } else if (k0 + BN > S || (p.causal && k0 + BN - 1 > r0 + diag)) {
           int vis = S - 1 - k0;
           if (p.causal) vis = imin(vis, row + diag - k0);
           vis -= 4 * hf;
@@ -511,7 +553,11 @@ __global__ __launch_bounds__(256 * KG, 2) void flash_f32_kernel(FlashParams p, i
     }
     if (failing(7)) {
       failed |= 1u << pass;
-      continue;
+      if constexpr (!WIN) continue;
+    }
+    if constexpr (WIN) {  // the 32-bit kernel does failed blocks
+      if (threadIdx.x == 0) p.redo[(bw.b * p.heads + bw.h) * ((L + kBM - 1) / kBM) + bw.q0 / kBM] = (int32_t)failed;
+      if (failed) return;
     }
     float isv = 1.f / sv;
     if constexpr (KG == 2) {
@@ -561,13 +607,15 @@ __global__ __launch_bounds__(256 * KG, 2) void flash_f32_kernel(FlashParams p, i
               f32x4{o[d][4 * g] * f, o[d][4 * g + 1] * f, o[d][4 * g + 2] * f, o[d][4 * g + 3] * f};
     }
   }
-  if (grp == 1) return;  // the 32-bit pass takes one group (its barriers wait for the waves still running)
+  if (WIN || grp == 1) return;  // the 32-bit pass takes one group (its barriers wait for the waves still running)
+  if constexpr (!WIN) {
 #pragma unroll 1
   for (int pass = 0; pass < np; ++pass) {
     if (!(failed >> pass & 1)) continue;
     __syncthreads();
     const BlockWork bw = pair ? BlockWork{pw.b, pw.h, (pass ? pw.qb1 : pw.qb0) * kBM} : block_work(p, blockIdx.x);
 #include "ca_f32_pass.inc"
+  }
   }
 }
 

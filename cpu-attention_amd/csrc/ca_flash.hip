@@ -1315,6 +1315,39 @@ int flash_launch(const FlashParams& p, int E, int bf16, hipStream_t stream) {
 
 int64_t flash_window_bf16_splits(const WindowParams& p) { return win_plan(p).splits; }
 
+// fp32 window calls on split operands: past f32_exact's few keys, from as many blocks of 128
+// rows on as make up for the smaller blocks of the 32-bit kernel.  32-bit MFMAs / split, us:
+// E=128 48 blocks (window 300) 33.4 / 41.9, 60 (300) 46.9 / 42.9, 64 (600) 52 / 55, 64 (300) 47.1 /
+// 42.3; E=64 64 (511) 24 / 34, 80 (511) 40.2 / 34.7, 96 (255) 28.5 / 26.7, 112 (300) 29.4 / 29.0,
+// 144 (300) 27.3 / 29.2, 192 (300) 50 / 29.8; E=32 128 (300) 18.2 / 22.2, 384 (400) 55 / 35.5.
+// N=1 L=S=4096 H=32 E=128 window 1023 669 / 278, L=S=2048 331 / 137.
+int64_t flash_window_f32_blocks(const WindowParams& p, int E) {
+  const int64_t seen = (int64_t)p.left + p.right + 1 + p.sinks, blocks = p.batch * p.heads * cdiv(p.seq_q, kBM);
+  if (f32_exact(E, true, seen < p.seq_k ? seen : p.seq_k)) return 0;
+  return blocks >= (E == 128 ? 64 : (E == 64 ? 80 : 160)) ? blocks : 0;
+}
+
+template <int E>
+static int window_f32_launch(const WindowParams& p, int64_t blocks, hipStream_t stream) {
+  // Two key groups where a CU gets at most one block (E = 32: two; one group / two, us: E=32 384
+  // blocks 40.6 / 35.5, 512 40.8 / 35.7; E=64 192 36.5 / 29.8, 384 45.2 / 53.7; E=128 192 52.9 /
+  // 44.1, 320 86.7 / 92.7).
+  if (blocks <= (E == 32 ? 512 : 256))
+    return launch_lds(flash_f32_kernel<E, 2, false, WindowParams>, blocks, 512, F32Cfg<E>::lds_bytes(2), p, stream, 1, 0);
+  return launch_lds(flash_f32_kernel<E, 1, false, WindowParams>, blocks, 256, F32Cfg<E>::lds_bytes(1), p, stream, 1, 0);
+}
+
+int flash_window_split_launch(const WindowParams& p, int E, hipStream_t stream) {
+  const int64_t blocks = flash_window_f32_blocks(p, E);
+  if (blocks > 0x7fffffff || !window_fits(p, E, 4)) return CA_DECLINED;
+  switch (E) {
+    case 32: return window_f32_launch<32>(p, blocks, stream);
+    case 64: return window_f32_launch<64>(p, blocks, stream);
+    case 128: return window_f32_launch<128>(p, blocks, stream);
+  }
+  return CA_DECLINED;
+}
+
 int flash_window_bf16_launch(const WindowParams& p, int E, hipStream_t stream) {
   if (!window_fits(p, E, 2)) return CA_DECLINED;
   // Few keys: one wave per 32 rows with every key in registers, as flash_plan (whose

@@ -17,6 +17,10 @@
 // SPLIT: few rows over long windows; blockIdx.y takes a share of the tiles and leaves its
 // rows' partials (O, max, sum) for the combine kernel.
 //
+// Runs calls of few rows or few visible keys (flash_window_f32_blocks in ca_flash.hip says
+// which run on split operands) and, with p.redo, the 128-row blocks of the others whose
+// values those do not hold.
+//
 // Bound: the 32-bit MFMAs (157 TFLOP/s dense), either shape; masked parts of the window's
 // edge tiles are computed too.
 #include <type_traits>
@@ -61,6 +65,7 @@ __global__ __launch_bounds__(256, KW == 1 ? 2 : 1) void win_f32_kernel(WindowPar
   const uint32_t* qg = reinterpret_cast<const uint32_t*>(p.q) + b * p.qs[0] + h * p.qs[2];
   const uint32_t* kg = reinterpret_cast<const uint32_t*>(p.k) + b * p.ks[0] + h * p.ks[2];
   const uint32_t* vg = reinterpret_cast<const uint32_t*>(p.v) + b * p.vs[0] + h * p.vs[2];
+  if (KW == 1 && p.redo && !p.redo[bh * nqb + q0 / BM]) return;
   const WinTiles wt = win_tiles(p, q0, BM, BN);
   // The block's tiles [t0, t1) of the list.
   const int share = SPLIT ? (wt.n + (int)gridDim.y - 1) / (int)gridDim.y : wt.n;
@@ -242,8 +247,8 @@ __global__ __launch_bounds__(256, KW == 1 ? 2 : 1) void win_f32_kernel(WindowPar
   }
 }
 
-// How a call runs: key waves and rows per wave of its blocks, and splits of their tiles.
-// 128-row blocks where they give every CU one (E = 128, whose 128-key tiles leave one block
+// How a call in 32-bit MFMAs runs: key waves and rows per wave of its blocks, and splits of
+// their tiles (calls of many blocks get here by their few visible keys).  128-row blocks where they give every CU one (E = 128, whose 128-key tiles leave one block
 // per CU: nearly), else 32-row ones, else 16-row ones.  Measured (us, window 300 unless
 // noted, KW = 1 / KW = 4 RB = 32 / RB = 16): N=1 L=333 S=2500 window 512 H=12 E=64 67.5 /
 // 28.1 / 20.3; N=2 L=S=700 H=12 E=64 48.0 / 24.5 / 30.7; L=S=1536 H=16 E=64 48.6 / 43.7,
@@ -298,6 +303,14 @@ static int win_f32_launch_e(const WindowParams& p, hipStream_t stream) {
 
 int flash_window_f32_launch(const WindowParams& p, int E, hipStream_t stream) {
   if (!window_fits(p, E, 4)) return CA_DECLINED;
+  if (p.redo) {
+    const WinF32Plan w{1, 32, p.batch * p.heads * cdiv(p.seq_q, 128), 1};
+    switch (E) {
+      case 32: return win_f32_launch_t<32, 1, 32, false>(p, w, stream);
+      case 64: return win_f32_launch_t<64, 1, 32, false>(p, w, stream);
+      case 128: return win_f32_launch_t<128, 1, 32, false>(p, w, stream);
+    }
+  }
   switch (E) {
     case 32: return win_f32_launch_e<32>(p, stream);
     case 64: return win_f32_launch_e<64>(p, stream);

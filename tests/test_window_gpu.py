@@ -35,8 +35,9 @@ def check(q, k, v, left, right, sinks, causal, scale=None):
 # (N, L, S, H, E, left, right, sinks, causal); bf16 routes by items = N H ceil(L / 128) and the
 # tiles a block can have: up to 256 keys one wave per 32 rows, then key groups past 8 tiles up to
 # 256 items, splits from 16 tiles up to 64 items and from 40 up to 170, one group otherwise.
-# fp32: 128-row blocks from 256 (E = 128: 192) of them, 32-row ones from 256, else 16-row
-# ones, split from 4 tiles of 128 keys where they leave half of the CUs idle.
+# fp32: split operands from 64 (E = 128), 80 (64) or 160 (32) 128-row blocks; 32-bit MFMAs in
+# 128-row blocks from 256 (E = 128: 192) of them, 32-row ones from 256, else 16-row ones, split
+# from 4 tiles of 128 keys where they leave half of the CUs idle.
 SHAPES = [
     (1, 1, 1, 1, 64, 0, 0, 0, True),
     (1, 1, 77, 2, 32, 3, 0, 2, True),
@@ -230,3 +231,91 @@ def test_bindings_agree(cuda, dtype):
         assert same_bytes(a, b)
     assert K.module().flash_window(rt, q, k[:, :, :2], v, None, True, 4, 0, 0) is None
     assert mod.flash_window(rt, q, k[:, :, :2], v, None, True, 4, 0, 0) is None
+
+
+# fp32 calls on split operands: two key groups and one at each head dim, rows of two blocks.
+SPLIT = [(2, 130, 500, 24, 64), (5, 130, 500, 32, 64), (2, 130, 500, 16, 128), (5, 130, 500, 32, 128),
+         (3, 130, 500, 32, 32), (9, 130, 500, 32, 32), (1, 1030, 1030, 10, 64), (1, 1100, 1100, 8, 128)]
+
+
+def _spoil(kind, q, k, v):
+    if kind == "sinks":            # keys with logits far above the others, values near none
+        k[:, :4] *= 6
+        v[:, :4] *= 2.0 ** -6
+    elif kind == "growing keys":   # past what the first tile's scale holds
+        k[:, 250:] *= 300
+        q *= 2.0 ** -8
+    elif kind == "wide column":
+        v[..., 5] *= 1e4
+    elif kind == "zero columns":
+        v[..., 3:17] = 0
+    elif kind == "late column":    # zeros in the first tiles only
+        v[:, :300, :, 7] = 0
+    elif kind == "zeros":
+        q[:, ::3] = 0
+        k[:, 40:90] = 0
+        v[:, 200:260] = 0
+    elif kind == "tiny":
+        q *= 1e-18
+        k *= 1e-18
+        v *= 1e-30
+    elif kind == "peaked":
+        q *= 30
+    elif kind == "uneven":
+        g = torch.Generator().manual_seed(3)
+        k *= torch.randn(k.shape, generator=g).mul(1.5).exp().to(k.device)
+        v *= torch.randn(v.shape, generator=g).mul(2).exp().to(v.device)
+    elif kind == "late nan":       # seen by the last rows only
+        v[0, -1, 1, 2] = float("nan")
+        k[0, -2, 0, 1] = float("inf")
+
+
+@pytest.mark.parametrize("shape", SPLIT, ids=lambda s: "-".join(map(str, s)))
+@pytest.mark.parametrize("kind", ["normal", "sinks", "growing keys", "wide column", "zero columns", "late column", "zeros",
+                                  "tiny", "peaked", "uneven", "late nan"])
+def test_fp32_values_of_every_size(cuda, shape, kind):
+    """The split operands hold values near their tile's largest; blocks where that costs a row
+    too much are done in 32-bit MFMAs.  Beside fp32's own errors there are the quanta of values
+    whose low half is subnormal: q', k', v', p' (scaled) are each off by at most 2^-25.
+      V's: in a dim, 2^-25 sum p'.  The kernel keeps a block only if top^2 >= 2^10 sum p' (top:
+        the row's largest |O'|), and p' <= 2^14, so sum p' <= sqrt(n 2^14) top / 2^5: at most
+        2^-23 sqrt(n) top over n keys.
+      P's: 2^-25 sum |v'| <= 2^-25 sqrt(n) sqrt(sum v'^2), and top^2 >= sum v'^2 / 2^6: at most
+        2^-22 sqrt(n) top, n the keys staged (the rows' and up to 191 around them).
+      the logits': c 2^-25 E (2^11 + |k'|), and c max(2^11, |k'|) <= max(1, X / 2) / 2 for a
+        logit of X log2 units: at most E 2^-25 max(1, X / 2), X / 2 times it within fp32's own
+        logit term, once it in numerator and denominator each: E 2^-24.
+    top is at most the largest sum p |v| of a dim."""
+    N, L, S, H, E = shape
+    q, k, v = inputs(N, L, S, H, E, torch.float32, seed=E + H)
+    _spoil(kind, q, k, v)
+    out = C.flash_attn_window_func(q, k, v, window_size=(270, 0), sink_tokens=4, causal=True)
+    ref = R.window(values(q), values(k), values(v), E ** -0.5, 270, 0, 4, True)
+    n = 275 + 191
+    bound = ref.bound("fp32", False) + E * 2.0 ** -24 * ref.size \
+        + (2.0 ** -23 + 2.0 ** -22) * n ** 0.5 * np.where(np.isfinite(ref.size), ref.size, 0).max(-1, keepdims=True)
+    got, nan = values(out), np.isnan(ref.out)
+    assert np.array_equal(np.isnan(got), nan)
+    fine = np.isfinite(ref.out)
+    assert np.array_equal(got[~fine & ~nan], ref.out[~fine & ~nan])
+    assert np.all(np.abs(got - ref.out)[fine] <= bound[fine]), np.max((np.abs(got - ref.out) / bound)[fine])
+
+
+def test_fp32_split_operands_captured(cuda):
+    """Replays of a call whose blocks stay on the split operands in one and are redone in the
+    next, a workspace of any contents."""
+    N, L, S, H, E = SPLIT[0]
+    q, k, v = inputs(N, L, S, H, E, torch.float32)
+
+    def call():
+        return C.flash_attn_window_func(q, k, v, window_size=(270, 0), sink_tokens=4, causal=True)
+
+    graph, out = capture(call)
+    for i, kind in enumerate(("normal", "wide column", "normal", "late nan", "normal")):
+        for x, y in zip((q, k, v), inputs(N, L, S, H, E, torch.float32, seed=i)):
+            x.copy_(y)
+        _spoil(kind, q, k, v)
+        want = call()
+        graph.replay()
+        torch.cuda.synchronize()
+        assert same_bytes(out, want)
