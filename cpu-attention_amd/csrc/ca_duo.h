@@ -658,21 +658,37 @@ __global__ __launch_bounds__(256 * KG, (DuoCfg<E, KG>::WAVES)) void flash_duo_ke
 }
 
 // How a window call runs: kg key groups and the splits of its blocks' tiles (1: none), by
-// duo_plan's lines with T the most tiles that a block walks.
+// duo_plan's lines with T the most tiles that a block walks, and pairs of blocks where the
+// window is most of the keys.  Unpaired / pairs, us, L=S, window 1/2, 0.7 and 0.95 of it: E=128
+// N=4 L=1024 H=32 (1024 items) 51.1 / 47.5, 60.6 / 48.5, 60.4 / 48.9, N=4 L=2048 H=32 150 / 144,
+// 166 / 154, 172 / 161, N=1 L=4096 H=16 (512) 65 / 75, 83 / 76, 103 / 78; E=64 N=2 L=4096 H=32 138 /
+// 149, 166 / 161, 187 / 165, N=8 L=700 H=16 (768) 20.5 / 27.7, 21.1 / 27.2, 21.2 / 25.2.  (Half:
+// with other inputs each call, N=4 L=2048 H=32 E=128 146 / 148.)
 struct WinPlan {
   int kg;
   int64_t items, splits;
+  bool pair;
+  int64_t gx;
 };
-inline WinPlan win_plan(const WindowParams& p) {
+inline WinPlan win_plan(const WindowParams& p, int E) {
   constexpr int BM = DuoCfg<64, 1>::BM, BN = DuoCfg<64, 1>::BN;
-  WinPlan w{1, p.batch * p.heads * cdiv(p.seq_q, BM), 1};
+  const int64_t nqb = cdiv(p.seq_q, BM);
+  WinPlan w{1, p.batch * p.heads * nqb, 1, false, p.batch * p.heads * nqb};
   const int64_t T = win_most_tiles(p, BM, BN);
   if (w.items <= 64 ? T >= 16 : (w.items <= 85 ? T >= 32 : w.items <= 170 && T >= 40)) {
     w.splits = (w.items > 85 || (w.items > 64 && T >= 96) ? 512 : 256) / w.items;
     w.splits = w.splits < T / 4 ? w.splits : T / 4;
     w.splits = w.splits < kTiledMaxSplits ? w.splits : kTiledMaxSplits;  // what the combine merges
   }
-  if (w.splits <= 1 && w.items <= 256 && T > 8) w.kg = 2;
+  if (w.splits > 1) return w;
+  if (w.items <= 256) {
+    w.kg = T > 8 ? 2 : 1;
+  } else if (E == 128 ? win_triangle(p, w.items > 512 ? 6 : 7) && (w.items > 512 || T >= 12)
+                      : win_triangle(p, 7) && w.items > 1024) {
+    w.kg = w.items <= 512 && T >= 32 ? 2 : 1;
+    w.pair = true;
+    w.gx = p.batch * p.heads * ((nqb + 1) / 2);
+  }
   return w;
 }
 
@@ -680,14 +696,14 @@ template <int E>
 static int win_launch(const WindowParams& p, hipStream_t stream) {
   using C1 = DuoCfg<E, 1>;
   using C2 = DuoCfg<E, 2>;
-  const WinPlan w = win_plan(p);
+  const WinPlan w = win_plan(p, E);
   if (w.splits > 1) {
     const int st = launch_lds(flash_duo_kernel<E, 1, true, WindowParams>, w.items, 256, C1::LDS_BYTES, p, stream, w.splits, 0);
     return st == CA_OK ? flash_combine_launch(p, E, true, w.splits, stream) : st;
   }
   if (w.kg == 2)
-    return launch_lds(flash_duo_kernel<E, 2, false, WindowParams>, w.items, 512, C2::LDS_BYTES, p, stream, 1, 0);
-  return launch_lds(flash_duo_kernel<E, 1, false, WindowParams>, w.items, 256, C1::LDS_BYTES, p, stream, 1, 0);
+    return launch_lds(flash_duo_kernel<E, 2, false, WindowParams>, w.gx, 512, C2::LDS_BYTES, p, stream, 1, (int)w.pair);
+  return launch_lds(flash_duo_kernel<E, 1, false, WindowParams>, w.gx, 256, C1::LDS_BYTES, p, stream, 1, (int)w.pair);
 }
 
 template <int E>

@@ -1313,7 +1313,7 @@ int flash_launch(const FlashParams& p, int E, int bf16, hipStream_t stream) {
   return CA_DECLINED;
 }
 
-int64_t flash_window_bf16_splits(const WindowParams& p) { return win_plan(p).splits; }
+int64_t flash_window_bf16_splits(const WindowParams& p) { return win_plan(p, 128).splits; }  // not E's
 
 // fp32 window calls on split operands: past f32_exact's few keys, from as many blocks of 128
 // rows on as make up for the smaller blocks of the 32-bit kernel.  32-bit MFMAs / split, us:

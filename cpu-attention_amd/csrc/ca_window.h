@@ -77,6 +77,13 @@ __host__ __device__ inline int64_t win_most_tiles(const WindowParams& p, int bm,
   return all < some ? all : some;
 }
 
+// Whether the first blocks have less to do than the last ones, as in a causal call of fewer
+// than twice as many keys as rows, over a window of `tenths` tenths of the keys or more:
+// pairs of blocks do even it out then.
+inline bool win_triangle(const WindowParams& p, int tenths) {
+  return p.right < p.seq_q - 1 && p.seq_k < 2 * p.seq_q && 10 * ((int64_t)p.left + 1) >= tenths * p.seq_k;
+}
+
 // Whether the row at position pos sees key j (of 0 .. S - 1).
 __host__ __device__ inline bool win_sees(const WindowParams& p, int pos, int j) {
   return j <= (int64_t)pos + p.right && (j >= (int64_t)pos - p.left || j < p.sinks);

@@ -319,3 +319,22 @@ def test_fp32_split_operands_captured(cuda):
         graph.replay()
         torch.cuda.synchronize()
         assert same_bytes(out, want)
+
+
+@pytest.mark.parametrize("dtype", DTYPES, ids=NAME.get)
+@pytest.mark.parametrize("shape", [(1, 1100, 1100, 60, 128, 800, 0, 4), (1, 1100, 1300, 57, 128, 1200, 3, 0),
+                                   (1, 2100, 2100, 16, 128, 1700, 0, 4), (1, 1990, 1990, 17, 128, 1500, 0, 70),
+                                   (8, 260, 260, 50, 64, 220, 0, 4), (7, 390, 400, 40, 32, 300, 20, 1)],
+                         ids=lambda s: "-".join(map(str, s)))
+def test_windows_of_most_keys(cuda, dtype, shape):
+    """Blocks in pairs, an odd one among them, of one and of two key groups."""
+    N, L, S, H, E, left, right, sinks = shape
+    check(*inputs(N, L, S, H, E, dtype, seed=L), left, right, sinks, False)
+
+
+def test_windows_of_most_keys_redo_rows(cuda):
+    for N, L, H, E, left in ((1, 1100, 60, 128, 800), (8, 260, 50, 64, 220)):
+        q, k, v = inputs(N, L, L, H, E, BF16, seed=L)
+        v[0, left // 2, 1, 3] = float("inf")
+        k[0, L - 9, 0, 2] = float("nan")
+        check(q, k, v, left, 0, 4, True)
