@@ -327,18 +327,17 @@ static WindowParams window_params(const FlashParams& f, const WindowSides& w) {
   return p;
 }
 
-// What a window call's workspace holds: the partials of `slots` (row, split) pairs, or the
-// words of `blocks` blocks (fp32 on split operands).
+// What a window call's workspace holds: the partials of `slots` (row, split) pairs, then the
+// `words` of an fp32 call on split operands.
 struct WindowSpace {
-  int64_t slots, blocks, bytes;
+  int64_t splits, slots, words, bytes;
 };
 static WindowSpace window_space(const WindowParams& p, int64_t head_dim, int32_t dtype) {
-  WindowSpace w{0, dtype == CA_BF16 ? 0 : flash_window_f32_blocks(p, (int)head_dim), 0};
-  if (w.blocks == 0) {
-    const int64_t splits = dtype == CA_BF16 ? flash_window_bf16_splits(p) : flash_window_f32_splits(p, (int)head_dim);
-    if (splits > 1) w.slots = p.batch * p.heads * p.seq_q * splits;
-  }
-  w.bytes = w.slots * (head_dim + 2) * 4 + w.blocks * 4;
+  const WinF32Blocks f = dtype == CA_BF16 ? WinF32Blocks{0, 1, false} : flash_window_f32_blocks(p, (int)head_dim);
+  WindowSpace w{f.splits, 0, f.blocks * f.splits, 0};
+  if (f.blocks == 0) w.splits = dtype == CA_BF16 ? flash_window_bf16_splits(p) : flash_window_f32_splits(p, (int)head_dim);
+  if (w.splits > 1) w.slots = p.batch * p.heads * p.seq_q * w.splits;
+  w.bytes = w.slots * (head_dim + 2) * 4 + w.words * 4;
   return w;
 }
 
@@ -397,11 +396,14 @@ extern "C" int ca_flash_window(const ca_flash_window_args* wa, void* stream) {
     p.part_acc = static_cast<float*>(a->workspace);
     p.part_ml = p.part_acc + ws.slots * a->head_dim;
     p.workspace_bytes = a->workspace_bytes;
-    if (ws.blocks > 0) p.redo = static_cast<int32_t*>(a->workspace);
+    if (ws.words > 0) {
+      p.redo = reinterpret_cast<int32_t*>(p.part_ml + 2 * ws.slots);
+      p.redo_splits = (int32_t)ws.splits;
+    }
   }
   hipStream_t st = static_cast<hipStream_t>(stream);
   if (a->dtype == CA_BF16) return flash_window_bf16_launch(p, (int)a->head_dim, st);
-  if (ws.blocks > 0) {
+  if (ws.words > 0) {
     const int r = flash_window_split_launch(p, (int)a->head_dim, st);
     if (r != CA_OK) return r;
   }

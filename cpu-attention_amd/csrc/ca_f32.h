@@ -183,7 +183,6 @@ inline bool f32_exact(int E, bool causal, int64_t seq_k) {
 template <int E, int KG, bool SPLIT, class P = FlashParams>
 __global__ __launch_bounds__(256 * KG, 2) void flash_f32_kernel(P p, int pair) {
   constexpr bool WIN = std::is_same<P, WindowParams>::value;
-  static_assert(!WIN || !SPLIT, "window calls are not split");
   using C = F32Cfg<E>;
   constexpr int BN = C::BN, PL = C::PL, TB = C::TB, CH = C::CH, NS = E / 16, ND = E / 32;
   extern __shared__ __attribute__((aligned(1024))) char f32_smem[];
@@ -222,10 +221,14 @@ __global__ __launch_bounds__(256 * KG, 2) void flash_f32_kernel(P p, int pair) {
     const float* vg = reinterpret_cast<const float*>(p.v) + bw.b * p.vs[0] + bw.h * p.vs[2];
     const int r0 = (int)bw.q0 + 32 * wv, row = r0 + li;
     WinTiles wt{};
+    int t0 = 0, t1 = 0;  // WIN: the block's tiles of the list
     F32Keys kr;
     if constexpr (WIN) {
       wt = win_tiles(p, (int)bw.q0, kBM, BN);
-      kr = F32Keys{0, 0, wt.n};
+      const int share = (wt.n + splits - 1) / splits;
+      t0 = imin(sp * share, wt.n);
+      t1 = imin(t0 + share, wt.n);
+      kr = F32Keys{0, 0, t1 - t0};
     } else {
       kr = f32_keys(p, bw.q0, SPLIT, sp, splits);
     }
@@ -241,8 +244,8 @@ __global__ __launch_bounds__(256 * KG, 2) void flash_f32_kernel(P p, int pair) {
     const int kstep = (int)(RI * p.ks[1] * 4), vstep = (int)(RI * p.vs[1] * 4);
     // WIN: round t's first key.  A group without a first tile takes the last one's scales.
     auto win_k0 = [&](int t) __attribute__((always_inline)) {
-      const int i = t * KG + grp;
-      return i < wt.n ? win_key0(wt, i, BN) : (t == 0 ? win_key0(wt, wt.n - 1, BN) : S);
+      const int i = t0 + t * KG + grp;
+      return i < t1 ? win_key0(wt, i, BN) : (t == 0 ? win_key0(wt, t1 - 1, BN) : S);
     };
     auto load_one = [&](const float* g, int64_t stride, int off, int step, int t, u32x4 (&x)[CH]) __attribute__((always_inline)) {
       int64_t k0 = kbeg + ((int64_t)t * KG + grp) * BN;
@@ -436,7 +439,7 @@ __global__ __launch_bounds__(256 * KG, 2) void flash_f32_kernel(P p, int pair) {
       bool mine = k0 < kend_w && (KG == 1 || t * KG + grp < kr.nkt);
       if constexpr (WIN) {
         k0 = win_k0(t);
-        mine = r0 < L && t * KG + grp < wt.n && k0 <= r0 + 31 + diag + p.right &&
+        mine = r0 < L && t0 + t * KG + grp < t1 && k0 <= r0 + 31 + diag + p.right &&
                (k0 + BN - 1 >= r0 + diag - p.left || k0 < p.sinks);
       }
       f32x16 st = f32x16{}, sx = f32x16{};
@@ -551,13 +554,14 @@ __global__ __launch_bounds__(256 * KG, 2) void flash_f32_kernel(P p, int pair) {
         ok &= kt < 0x7c00u && vs < INFINITY && top * top >= fmaf(lt, kF32RowSum, vs * (CH * kF32RowKeys)) &&
               c * kv <= kF32Logit * fmaxf(1.f, 0.5f * fabsf(m + kF32Lift));
     }
-    if (failing(7)) {
-      failed |= 1u << pass;
-      if constexpr (!WIN) continue;
-    }
     if constexpr (WIN) {  // the 32-bit kernel does failed blocks
-      if (threadIdx.x == 0) p.redo[(bw.b * p.heads + bw.h) * ((L + kBM - 1) / kBM) + bw.q0 / kBM] = (int32_t)failed;
-      if (failed) return;
+      const bool bad = failing(7);
+      const int64_t block = (bw.b * p.heads + bw.h) * ((L + kBM - 1) / kBM) + bw.q0 / kBM;
+      if (threadIdx.x == 0) p.redo[block * splits + sp] = bad;
+      if (bad) continue;
+    } else if (failing(7)) {
+      failed |= 1u << pass;
+      continue;
     }
     float isv = 1.f / sv;
     if constexpr (KG == 2) {

@@ -1315,35 +1315,53 @@ int flash_launch(const FlashParams& p, int E, int bf16, hipStream_t stream) {
 
 int64_t flash_window_bf16_splits(const WindowParams& p) { return win_plan(p, 128).splits; }  // not E's
 
-// fp32 window calls on split operands: past f32_exact's few keys, from as many blocks of 128
-// rows on as make up for the smaller blocks of the 32-bit kernel.  32-bit MFMAs / split, us:
+// fp32 window calls on split operands: past f32_exact's few keys and the few rows that
+// 16-row blocks serve, from as many blocks of 128 rows (times splits of their tiles) on as
+// make up for the smaller blocks of the 32-bit kernel.  32-bit MFMAs / split operands, us:
 // E=128 48 blocks (window 300) 33.4 / 41.9, 60 (300) 46.9 / 42.9, 64 (600) 52 / 55, 64 (300) 47.1 /
 // 42.3; E=64 64 (511) 24 / 34, 80 (511) 40.2 / 34.7, 96 (255) 28.5 / 26.7, 112 (300) 29.4 / 29.0,
 // 144 (300) 27.3 / 29.2, 192 (300) 50 / 29.8; E=32 128 (300) 18.2 / 22.2, 384 (400) 55 / 35.5.
-// N=1 L=S=4096 H=32 E=128 window 1023 669 / 278, L=S=2048 331 / 137.
-int64_t flash_window_f32_blocks(const WindowParams& p, int E) {
-  const int64_t seen = (int64_t)p.left + p.right + 1 + p.sinks, blocks = p.batch * p.heads * cdiv(p.seq_q, kBM);
-  if (f32_exact(E, true, seen < p.seq_k ? seen : p.seq_k)) return 0;
-  return blocks >= (E == 128 ? 64 : (E == 64 ? 80 : 160)) ? blocks : 0;
+// N=1 L=S=4096 H=32 E=128 window 1023 669 / 278, L=S=2048 331 / 137; L=16 rows N=8 S=2048 H=32
+// E=64 38 / 47, 17 rows 47.9 / 47.2, N=4 L=30 E=128 61 / 45.  Splits as the dense call's (L=256
+// S=4096 H=32 E=128 window 3900 226 -> 86, L=128 H=16 87 -> 42).  Pairs where the window is most of
+// the keys: unpaired / pairs, window 0.7 and 0.95 of L=S: E=128 N=4 L=1024 H=32 213 / 163, 233 /
+// 166, N=1 L=4096 H=16 323 / 252, 424 / 258; E=64 N=2 L=4096 H=32 555 / 564, 621 / 567, N=8 L=700 H=16
+// (768 blocks) 56 / 77, 60 / 76.
+WinF32Blocks flash_window_f32_blocks(const WindowParams& p, int E) {
+  const int64_t seen = (int64_t)p.left + p.right + 1 + p.sinks, nqb = cdiv(p.seq_q, kBM);
+  const WinF32Blocks none{0, 1, false};
+  if (p.seq_q <= kRowsMaxL || f32_exact(E, true, seen < p.seq_k ? seen : p.seq_k)) return none;
+  WinF32Blocks w{p.batch * p.heads * nqb, 1, false};
+  const int64_t most = 32 * win_most_tiles(p, kBM, 32);
+  w.splits = tiled_splits(p.batch, p.seq_q, most, p.heads, false, false);
+  if (w.blocks * w.splits < (E == 128 ? 64 : (E == 64 ? 80 : 160))) return none;
+  FlashParams f = p;
+  f.causal = 1;
+  w.pair = w.splits == 1 && win_triangle(p, 6) && (E == 128 || w.blocks >= 1024) && pair_blocks(f, nqb, false);
+  return w;
 }
 
 template <int E>
-static int window_f32_launch(const WindowParams& p, int64_t blocks, hipStream_t stream) {
+static int window_f32_launch(WindowParams p, const WinF32Blocks& w, hipStream_t stream) {
+  constexpr int lds = F32Cfg<E>::lds_bytes(1);
+  if (w.splits > 1) return launch_lds(flash_f32_kernel<E, 1, true, WindowParams>, w.blocks, 256, lds, p, stream, w.splits, 0);
+  p.causal = w.pair;  // pair_work's order
+  const int64_t gx = w.pair ? p.batch * p.heads * ((cdiv(p.seq_q, kBM) + 1) / 2) : w.blocks;
   // Two key groups where a CU gets at most one block (E = 32: two; one group / two, us: E=32 384
   // blocks 40.6 / 35.5, 512 40.8 / 35.7; E=64 192 36.5 / 29.8, 384 45.2 / 53.7; E=128 192 52.9 /
   // 44.1, 320 86.7 / 92.7).
-  if (blocks <= (E == 32 ? 512 : 256))
-    return launch_lds(flash_f32_kernel<E, 2, false, WindowParams>, blocks, 512, F32Cfg<E>::lds_bytes(2), p, stream, 1, 0);
-  return launch_lds(flash_f32_kernel<E, 1, false, WindowParams>, blocks, 256, F32Cfg<E>::lds_bytes(1), p, stream, 1, 0);
+  if (gx <= (E == 32 ? 512 : 256))
+    return launch_lds(flash_f32_kernel<E, 2, false, WindowParams>, gx, 512, F32Cfg<E>::lds_bytes(2), p, stream, 1, (int)w.pair);
+  return launch_lds(flash_f32_kernel<E, 1, false, WindowParams>, gx, 256, lds, p, stream, 1, (int)w.pair);
 }
 
 int flash_window_split_launch(const WindowParams& p, int E, hipStream_t stream) {
-  const int64_t blocks = flash_window_f32_blocks(p, E);
-  if (blocks > 0x7fffffff || !window_fits(p, E, 4)) return CA_DECLINED;
+  const WinF32Blocks w = flash_window_f32_blocks(p, E);
+  if (w.blocks > 0x7fffffff || !window_fits(p, E, 4)) return CA_DECLINED;
   switch (E) {
-    case 32: return window_f32_launch<32>(p, blocks, stream);
-    case 64: return window_f32_launch<64>(p, blocks, stream);
-    case 128: return window_f32_launch<128>(p, blocks, stream);
+    case 32: return window_f32_launch<32>(p, w, stream);
+    case 64: return window_f32_launch<64>(p, w, stream);
+    case 128: return window_f32_launch<128>(p, w, stream);
   }
   return CA_DECLINED;
 }

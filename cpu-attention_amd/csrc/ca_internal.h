@@ -125,7 +125,9 @@ struct FlashParams {
 // left, right and sinks lie in 0 .. 2^30 (an open side: 2^30), c > 0; `causal` is not read.
 struct WindowParams : FlashParams {
   int32_t left, right, sinks;
-  int32_t* redo;  // fp32 on split operands: per (batch, head, 128 rows), 1 for the 32-bit kernel to do
+  // fp32 on split operands: per (batch, head, 128 rows) and split, 1 for the 32-bit kernel to do.
+  int32_t* redo;
+  int32_t redo_splits;
 };
 
 // Calls with few query rows take the few-rows route (ca_rows.hip): up to 4 rows
@@ -347,9 +349,14 @@ int flash_small_launch(const FlashParams& p, const FlashPlan& plan, int head_dim
 // The prefill with a window and sinks: splits of the keys (1: no workspace), and launch.
 int64_t flash_window_bf16_splits(const WindowParams& p);
 int64_t flash_window_f32_splits(const WindowParams& p, int head_dim);
-// Blocks of 128 rows of an fp32 call on split operands (0: it runs in 32-bit MFMAs), each with
-// a word of p.redo; flash_window_f32_launch then does the blocks that ask for it.
-int64_t flash_window_f32_blocks(const WindowParams& p, int head_dim);
+// An fp32 window call on split operands: blocks of 128 rows (0: it runs in 32-bit MFMAs) and
+// splits of their tiles, in pairs or not.  Each block and split has a word of p.redo;
+// flash_window_f32_launch does those that ask for it, and merges the splits.
+struct WinF32Blocks {
+  int64_t blocks, splits;
+  bool pair;
+};
+WinF32Blocks flash_window_f32_blocks(const WindowParams& p, int head_dim);
 int flash_window_split_launch(const WindowParams& p, int head_dim, hipStream_t stream);
 int flash_window_bf16_launch(const WindowParams& p, int head_dim, hipStream_t stream);
 int flash_window_small_launch(const WindowParams& p, int head_dim, hipStream_t stream);

@@ -65,7 +65,7 @@ __global__ __launch_bounds__(256, KW == 1 ? 2 : 1) void win_f32_kernel(WindowPar
   const uint32_t* qg = reinterpret_cast<const uint32_t*>(p.q) + b * p.qs[0] + h * p.qs[2];
   const uint32_t* kg = reinterpret_cast<const uint32_t*>(p.k) + b * p.ks[0] + h * p.ks[2];
   const uint32_t* vg = reinterpret_cast<const uint32_t*>(p.v) + b * p.vs[0] + h * p.vs[2];
-  if (KW == 1 && p.redo && !p.redo[bh * nqb + q0 / BM]) return;
+  if (KW == 1 && p.redo && !p.redo[((int64_t)bh * nqb + q0 / BM) * gridDim.y + blockIdx.y]) return;
   const WinTiles wt = win_tiles(p, q0, BM, BN);
   // The block's tiles [t0, t1) of the list.
   const int share = SPLIT ? (wt.n + (int)gridDim.y - 1) / (int)gridDim.y : wt.n;
@@ -249,7 +249,8 @@ __global__ __launch_bounds__(256, KW == 1 ? 2 : 1) void win_f32_kernel(WindowPar
 
 // How a call in 32-bit MFMAs runs: key waves and rows per wave of its blocks, and splits of
 // their tiles (calls of many blocks get here by their few visible keys).  128-row blocks where they give every CU one (E = 128, whose 128-key tiles leave one block
-// per CU: nearly), else 32-row ones, else 16-row ones.  Measured (us, window 300 unless
+// per CU: nearly), else 32-row ones, else 16-row ones, and none of more rows than twice the
+// call's (N=8 L=1 H=32 E=128 window 1023 164 -> 66).  Measured (us, window 300 unless
 // noted, KW = 1 / KW = 4 RB = 32 / RB = 16): N=1 L=333 S=2500 window 512 H=12 E=64 67.5 /
 // 28.1 / 20.3; N=2 L=S=700 H=12 E=64 48.0 / 24.5 / 30.7; L=S=1536 H=16 E=64 48.6 / 43.7,
 // E=128 81.1 / 82.7; N=2 L=S=1024 H=16 E=128 81.8 / 102.  16-row blocks that leave half of the
@@ -264,9 +265,9 @@ constexpr int64_t kMinShare = 2;
 static WinF32Plan win_f32_plan(const WindowParams& p, int E) {
   const int64_t bh = p.batch * p.heads;
   WinF32Plan w{1, 32, bh * cdiv(p.seq_q, 128), 1};
-  if (w.blocks > (E == 128 ? 192 : 256)) return w;
+  if (w.blocks > (E == 128 ? 192 : 256) && p.seq_q > 32) return w;
   w = WinF32Plan{4, 32, bh * cdiv(p.seq_q, 32), 1};
-  if (w.blocks > 256) return w;
+  if (w.blocks > 256 && p.seq_q > 16) return w;
   w = WinF32Plan{4, 16, bh * cdiv(p.seq_q, 16), 1};
   const int64_t T = win_most_tiles(p, 16, 128), by_tiles = T / kMinShare;
   if (w.blocks > 0 && w.blocks <= 128 && by_tiles >= 2) w.splits = 256 / w.blocks < by_tiles ? 256 / w.blocks : by_tiles;
@@ -301,14 +302,21 @@ static int win_f32_launch_e(const WindowParams& p, hipStream_t stream) {
   return w.rb == 32 ? win_f32_launch_t<E, 4, 32, false>(p, w, stream) : win_f32_launch_t<E, 4, 16, false>(p, w, stream);
 }
 
+template <int E>
+static int win_f32_redo(const WindowParams& p, hipStream_t stream) {
+  const WinF32Plan w{1, 32, p.batch * p.heads * cdiv(p.seq_q, 128), p.redo_splits};
+  if (w.splits == 1) return win_f32_launch_t<E, 1, 32, false>(p, w, stream);
+  const int st = win_f32_launch_t<E, 1, 32, true>(p, w, stream);
+  return st == CA_OK ? flash_combine_launch(p, E, false, w.splits, stream) : st;
+}
+
 int flash_window_f32_launch(const WindowParams& p, int E, hipStream_t stream) {
   if (!window_fits(p, E, 4)) return CA_DECLINED;
   if (p.redo) {
-    const WinF32Plan w{1, 32, p.batch * p.heads * cdiv(p.seq_q, 128), 1};
     switch (E) {
-      case 32: return win_f32_launch_t<32, 1, 32, false>(p, w, stream);
-      case 64: return win_f32_launch_t<64, 1, 32, false>(p, w, stream);
-      case 128: return win_f32_launch_t<128, 1, 32, false>(p, w, stream);
+      case 32: return win_f32_redo<32>(p, stream);
+      case 64: return win_f32_redo<64>(p, stream);
+      case 128: return win_f32_redo<128>(p, stream);
     }
   }
   switch (E) {

@@ -270,13 +270,11 @@ def _spoil(kind, q, k, v):
         k[0, -2, 0, 1] = float("inf")
 
 
-@pytest.mark.parametrize("shape", SPLIT, ids=lambda s: "-".join(map(str, s)))
-@pytest.mark.parametrize("kind", ["normal", "sinks", "growing keys", "wide column", "zero columns", "late column", "zeros",
-                                  "tiny", "peaked", "uneven", "late nan"])
-def test_fp32_values_of_every_size(cuda, shape, kind):
-    """The split operands hold values near their tile's largest; blocks where that costs a row
-    too much are done in 32-bit MFMAs.  Beside fp32's own errors there are the quanta of values
-    whose low half is subnormal: q', k', v', p' (scaled) are each off by at most 2^-25.
+def _check_split(q, k, v, left, parts):
+    """A call on split operands: they hold values near their tile's largest; blocks where that
+    costs a row too much are done in 32-bit MFMAs.  Beside fp32's own errors there are the
+    quanta of values whose low half is subnormal: q', k', v', p' (scaled) are each off by at
+    most 2^-25.
       V's: in a dim, 2^-25 sum p'.  The kernel keeps a block only if top^2 >= 2^10 sum p' (top:
         the row's largest |O'|), and p' <= 2^14, so sum p' <= sqrt(n 2^14) top / 2^5: at most
         2^-23 sqrt(n) top over n keys.
@@ -285,20 +283,43 @@ def test_fp32_values_of_every_size(cuda, shape, kind):
       the logits': c 2^-25 E (2^11 + |k'|), and c max(2^11, |k'|) <= max(1, X / 2) / 2 for a
         logit of X log2 units: at most E 2^-25 max(1, X / 2), X / 2 times it within fp32's own
         logit term, once it in numerator and denominator each: E 2^-24.
-    top is at most the largest sum p |v| of a dim."""
-    N, L, S, H, E = shape
-    q, k, v = inputs(N, L, S, H, E, torch.float32, seed=E + H)
-    _spoil(kind, q, k, v)
-    out = C.flash_attn_window_func(q, k, v, window_size=(270, 0), sink_tokens=4, causal=True)
-    ref = R.window(values(q), values(k), values(v), E ** -0.5, 270, 0, 4, True)
-    n = 275 + 191
-    bound = ref.bound("fp32", False) + E * 2.0 ** -24 * ref.size \
-        + (2.0 ** -23 + 2.0 ** -22) * n ** 0.5 * np.where(np.isfinite(ref.size), ref.size, 0).max(-1, keepdims=True)
+    top is at most the largest sum p |v| of a dim, in each of the `parts` (key groups or
+    splits) that share the keys: sqrt(parts n) over all."""
+    N, L, H, E = q.shape
+    out = C.flash_attn_window_func(q, k, v, window_size=(left, 0), sink_tokens=4, causal=True)
+    ref = R.window(values(q), values(k), values(v), E ** -0.5, left, 0, 4, True)
+    n = left + 5 + 191
+    top = np.where(np.isfinite(ref.size), ref.size, 0).max(-1, keepdims=True)
+    bound = ref.bound("fp32", False) + E * 2.0 ** -24 * ref.size + (2.0 ** -23 + 2.0 ** -22) * (parts * n) ** 0.5 * top
     got, nan = values(out), np.isnan(ref.out)
     assert np.array_equal(np.isnan(got), nan)
     fine = np.isfinite(ref.out)
     assert np.array_equal(got[~fine & ~nan], ref.out[~fine & ~nan])
     assert np.all(np.abs(got - ref.out)[fine] <= bound[fine]), np.max((np.abs(got - ref.out) / bound)[fine])
+
+
+KINDS = ["normal", "sinks", "growing keys", "wide column", "zero columns", "late column", "zeros", "tiny", "peaked", "uneven",
+         "late nan"]
+
+
+@pytest.mark.parametrize("shape", SPLIT, ids=lambda s: "-".join(map(str, s)))
+@pytest.mark.parametrize("kind", KINDS)
+def test_fp32_values_of_every_size(cuda, shape, kind):
+    N, L, S, H, E = shape
+    q, k, v = inputs(N, L, S, H, E, torch.float32, seed=E + H)
+    _spoil(kind, q, k, v)
+    _check_split(q, k, v, 270, 2)
+
+
+# Few blocks over long windows share their tiles out: 7, 11 and 11 splits.
+@pytest.mark.parametrize("shape", [(1, 256, 2000, 8, 64, 1900), (1, 130, 3001, 6, 128, 2800), (2, 100, 3001, 10, 32, 2800)],
+                         ids=lambda s: "-".join(map(str, s)))
+@pytest.mark.parametrize("kind", KINDS)
+def test_fp32_splits_of_every_size(cuda, shape, kind):
+    N, L, S, H, E, left = shape
+    q, k, v = inputs(N, L, S, H, E, torch.float32, seed=E + H)
+    _spoil(kind, q, k, v)
+    _check_split(q, k, v, left, 11)
 
 
 def test_fp32_split_operands_captured(cuda):
@@ -338,3 +359,12 @@ def test_windows_of_most_keys_redo_rows(cuda):
         v[0, left // 2, 1, 3] = float("inf")
         k[0, L - 9, 0, 2] = float("nan")
         check(q, k, v, left, 0, 4, True)
+
+
+@pytest.mark.parametrize("dtype", DTYPES, ids=NAME.get)
+@pytest.mark.parametrize("shape", [(9, 1, 700, 32, 128, 500), (9, 16, 700, 32, 64, 500), (9, 17, 300, 32, 64, 260),
+                                   (9, 32, 300, 32, 128, 30), (17, 33, 90, 32, 32, 20)],
+                         ids=lambda s: "-".join(map(str, s)))
+def test_few_rows_of_many_sequences(cuda, dtype, shape):
+    N, L, S, H, E, left = shape
+    check(*inputs(N, L, S, H, E, dtype, seed=L), left, 0, 4, True)
