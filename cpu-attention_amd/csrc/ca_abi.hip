@@ -345,7 +345,7 @@ extern "C" int64_t ca_flash_window_workspace_bytes(int64_t batch, int64_t seq_q,
                                                    int64_t head_dim, int32_t dtype, int32_t causal, int64_t left,
                                                    int64_t right, int64_t sinks) {
   if (!dtype_ok(dtype) || !head_dim_ok(head_dim) || batch < 1 || num_heads < 1 || seq_q < 1 || seq_k < 1) return 0;
-  if (seq_q >= (1 << 30) || seq_k >= (1 << 30)) return 0;  // declined
+  if (seq_q > kWindowMaxSeq || seq_k > kWindowMaxSeq) return 0;  // declined
   const WindowSides w = window_sides(seq_q, seq_k, causal != 0, left, right, sinks);
   if (w.plain) return ca_flash_workspace_bytes(batch, seq_q, seq_k, num_heads, head_dim, dtype);
   FlashParams f{};
@@ -361,7 +361,7 @@ extern "C" int ca_flash_window(const ca_flash_window_args* wa, void* stream) {
   const ca_flash_args* a = &wa->flash;
   if (!dtype_ok(a->dtype) || !head_dim_ok(a->head_dim) || wa->sinks < 0 || !scale_ok(a->scale)) return CA_DECLINED;
   if (a->batch < 0 || a->num_heads <= 0 || a->seq_q < 1 || a->seq_k < 1) return CA_DECLINED;
-  if (a->seq_q >= (1 << 30) || a->seq_k >= (1 << 30)) return CA_DECLINED;
+  if (a->seq_q > kWindowMaxSeq || a->seq_k > kWindowMaxSeq) return CA_DECLINED;
   const WindowSides w = window_sides(a->seq_q, a->seq_k, a->causal != 0, wa->left, wa->right, wa->sinks);
   if (w.plain) {
     ca_flash_args f = *a;

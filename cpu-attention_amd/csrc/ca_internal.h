@@ -123,6 +123,9 @@ struct FlashParams {
 // A prefill with a sliding window and sinks: row i (position i + seq_k - seq_q = pos) sees
 // keys pos - left .. pos + right, and of the first `sinks` those up to pos + right.
 // left, right and sinks lie in 0 .. 2^30 (an open side: 2^30), c > 0; `causal` is not read.
+// Keys and rows of a window call: a position (of rows past the last one in its block, too) plus
+// an open side (2^30) stays within 31 bits.
+constexpr int64_t kWindowMaxSeq = ((int64_t)1 << 30) - 1024;
 struct WindowParams : FlashParams {
   int32_t left, right, sinks;
   // fp32 on split operands: per (batch, head, 128 rows) and split, 1 for the 32-bit kernel to do.

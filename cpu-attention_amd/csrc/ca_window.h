@@ -67,7 +67,7 @@ inline bool window_fits(const WindowParams& p, int E, int esize) {
   int64_t ts = p.ks[1] > p.vs[1] ? p.ks[1] : p.vs[1];
   if (p.qs[1] > ts) ts = p.qs[1];
   return p.qs[1] >= 0 && p.ks[1] >= 0 && p.vs[1] >= 0 && 64 * (ts + E) * esize < ((int64_t)1 << 31) &&
-         p.seq_q < ((int64_t)1 << 30) && p.seq_k < ((int64_t)1 << 30);
+         p.seq_q <= kWindowMaxSeq && p.seq_k <= kWindowMaxSeq;
 }
 
 // The most tiles of any block: what the plans go by.

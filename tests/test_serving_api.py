@@ -369,3 +369,18 @@ def test_no_heads():
         C.flash_attn_window_func(q, q, q, window_size=(2, 0))
     with pytest.raises(ValueError, match="at least one head"):
         C.flash_attn_window_func(torch.zeros(1, 4, 2, 64), q, q, window_size=(2, 0))
+
+
+def test_window_positions_stay_within_31_bits():
+    """An empty batch, so that only the sizes are looked at."""
+    lib = K.load_library()
+    f = K.FlashWindowArgs(left=3, right=-1, sinks=0)
+    f.flash.seq_q, f.flash.num_heads, f.flash.head_dim, f.flash.dtype, f.flash.scale = 40, 2, 64, 1, 1.0
+    for seq_k, want in (((1 << 30) - 1024, K.CA_OK), ((1 << 30) - 1023, K.CA_DECLINED), ((1 << 30) - 1, K.CA_DECLINED)):
+        f.flash.seq_k = seq_k
+        assert lib.ca_flash_window(ctypes.byref(f), None) == want
+    d = K.DecodeWindowArgs(left=3, sinks=0, longest=12)
+    d.decode.num_heads, d.decode.head_dim, d.decode.page_size, d.decode.scale = 2, 64, 16, 1.0
+    assert lib.ca_decode_window(ctypes.byref(d), None) == K.CA_DECLINED
+    d.longest = 16
+    assert lib.ca_decode_window(ctypes.byref(d), None) == K.CA_OK
